@@ -40,6 +40,8 @@ pub const K_SGD_MOMENTUM: i32 = 7;
 pub const K_ADAM: i32 = 8;
 pub const K_SOFTMAX_XENT: i32 = 9;
 pub const K_MAXPOOL2D: i32 = 10;
+pub const K_TOKEN_LOGPROB: i32 = 11;
+pub const K_DISTILL_TOPK: i32 = 12;
 
 // eb200_reduce_op
 pub const R_NONE: i32 = 0;

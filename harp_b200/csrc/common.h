@@ -164,6 +164,9 @@ enum Impl {
     IMPL_SOFTMAX_XENT,    // log-softmax + cross-entropy, loss and logits gradient in one kernel
     IMPL_SIBLINGS,        // row reduce + column max + transposing copy of one [R, C] tensor in one pass
     IMPL_MAXPOOL,         // max_pool2d (stride = window) forward or gradient, optional fused ReLU
+    IMPL_TOKEN_LOGPROB,   // token log-probabilities, entropy, top alternatives of logits rows
+    IMPL_TOKEN_LOGPROB_GRAD,
+    IMPL_DISTILL_TOPK,    // distillation loss against a teacher's top logits, optionally with the logits gradient
 };
 
 struct GemmShape {
@@ -186,6 +189,21 @@ struct ConvShape {
     int N = 0, C = 0, H = 0, W = 0, Co = 0, KH = 0, KW = 0, pad = 0;
     int relu = 0, mode = EB200_GEMM_3XTF32, has_bias = 0, flip = 0, wgrad = 0, nchw = 0, g_nchw = 0, direct = 0;
 };
+
+// IMPL_TOKEN_LOGPROB*, IMPL_DISTILL_TOPK: [n, v] logits rows
+struct TokenShape {
+    long long n = 0;
+    int v = 0, k = 0;
+    long long pitch = 0, offset = 0;          // logits, elements
+    long long g_pitch = 0, g_offset = 0;      // gradient (or output 0 of a forward kernel: offset only)
+    int dtype = EB200_F32, id_dtype = EB200_I32, teacher_dtype = EB200_F32;
+    bool grad = false, entropy = false;
+    float scale = 1.f;
+    int cluster = 1;                          // CTAs that share a row
+    int lanes = 0;                            // > 0: short rows, that many lanes of a warp per row
+};
+
+constexpr int KMAX_OUT = 5;
 
 struct TransposeShape {
     // out[b][r][c] (contiguous) = in[b*sb + c*sc + r]  (input contiguous along r)
@@ -211,6 +229,7 @@ struct Plan {
     int fold_sh = 0, fold_sw = 0, fold_dh = 0, fold_dw = 0, fold_hout = 0, fold_wout = 0;
     int pool_flags = 0;                     // IMPL_MAXPOOL: 1 = ReLU on the taps, 2 = gradient
     TransposeShape tr;
+    TokenShape tok;
     int64_t scratch_bytes = 0;
     bool scratch_zero = false;    // the scratch must start at zero (set once, at kernel creation)
     int64_t algo_bytes = 0, algo_flops = 0;
@@ -225,6 +244,9 @@ struct Plan {
     int64_t in_numel[KMAX_IN] = {0};
     int out_dtype = 0;
     int64_t out_numel = 0;
+    int n_outputs = 1;            // outputs after the first: more_dtype / more_numel
+    int more_dtype[KMAX_OUT - 1] = {0};
+    int64_t more_numel[KMAX_OUT - 1] = {0};
     char name[64] = {0};
 };
 
@@ -252,6 +274,9 @@ long long siblings_scratch_floats(long long R, long long C);
 int launch_maxpool(Device* dev, const Plan& plan, const float* a, const float* b, const float* c, float* out);
 int launch_siblings(Device* dev, const Plan& plan, const KParams& p, const float* x, float* out, void* scratch);
 int launch_scan(Device* dev, const Plan& plan, const KParams& p, void* scratch);
+// in / out: device addresses of the descriptor's inputs and outputs, offsets not applied
+void token_variant(TokenShape* t, int sm_count);
+int launch_token(Device* dev, const Plan& plan, const void* const* in, void* const* out);
 int launch_gemm_simt(Device* dev, const Plan& plan, const float* a, const float* b, float* c, void* scratch);
 int launch_splitk_reduce(Device* dev, const GemmShape& g, const float* partials, float* c);
 bool gemm_tc_supported(const GemmShape& g);

@@ -58,7 +58,7 @@ static void fill_info(const Plan& plan, eb200_kernel_info* info) {
     strncpy(info->impl, plan.name, sizeof(info->impl) - 1);
     info->launches = plan.launches;
     info->specialised = plan.chain >= 0 || plan.impl == IMPL_TRANSPOSE || plan.impl == IMPL_SCATTER || plan.impl == IMPL_FOLD_GATHER ||
-                        plan.impl == IMPL_SGD || plan.impl == IMPL_SGD_MOMENTUM || plan.impl == IMPL_ADAM || plan.impl == IMPL_SOFTMAX_XENT || plan.impl == IMPL_MAXPOOL || plan.impl == IMPL_GEMM_SIMT || plan.impl == IMPL_GEMM_TC || plan.impl == IMPL_CONV2D || plan.impl == IMPL_GEMM_TALL || plan.impl == IMPL_CONV2D_WGRAD || plan.impl == IMPL_CONV2D_DIRECT || plan.impl == IMPL_CONV2D_DIRECT_WGRAD;
+                        plan.impl == IMPL_SGD || plan.impl == IMPL_SGD_MOMENTUM || plan.impl == IMPL_ADAM || plan.impl == IMPL_SOFTMAX_XENT || plan.impl == IMPL_MAXPOOL || plan.impl == IMPL_TOKEN_LOGPROB || plan.impl == IMPL_TOKEN_LOGPROB_GRAD || plan.impl == IMPL_DISTILL_TOPK || plan.impl == IMPL_GEMM_SIMT || plan.impl == IMPL_GEMM_TC || plan.impl == IMPL_CONV2D || plan.impl == IMPL_GEMM_TALL || plan.impl == IMPL_CONV2D_WGRAD || plan.impl == IMPL_CONV2D_DIRECT || plan.impl == IMPL_CONV2D_DIRECT_WGRAD;
     info->scratch_bytes = plan.scratch_bytes;
     info->algo_bytes = plan.algo_bytes;
     info->algo_flops = plan.algo_flops;
@@ -84,7 +84,7 @@ int eb200_kernel_launch(eb200_kernel* k, eb200_buffer* const* inputs, int n_inpu
     EB_REQUIRE(k && (inputs || !n_inputs) && outputs, EB200_ERR_INVALID, "null argument");
     const Plan& plan = k->plan;
     EB_REQUIRE(n_inputs == plan.n_inputs, EB200_ERR_INVALID, "kernel takes %d inputs, got %d", plan.n_inputs, n_inputs);
-    EB_REQUIRE(n_outputs == 1, EB200_ERR_INVALID, "kernel writes 1 output, got %d", n_outputs);
+    EB_REQUIRE(n_outputs == plan.n_outputs, EB200_ERR_INVALID, "kernel writes %d output%s, got %d", plan.n_outputs, plan.n_outputs == 1 ? "" : "s", n_outputs);
     Device* dev = k->dev;
     for (int i = 0; i < n_inputs; ++i) {
         EB_REQUIRE(inputs[i] && inputs[i]->dev == dev, EB200_ERR_INVALID, "input %d is null or lives on another device", i);
@@ -97,6 +97,11 @@ int eb200_kernel_launch(eb200_kernel* k, eb200_buffer* const* inputs, int n_inpu
         size_t need = (size_t)plan.out_numel * dtype_bytes(plan.out_dtype);
         EB_REQUIRE(ob->bytes >= need, EB200_ERR_BOUNDS, "output holds %zu bytes, kernel addresses %zu", ob->bytes, need);
     }
+    for (int j = 1; j < n_outputs; ++j) {
+        EB_REQUIRE(outputs[j] && outputs[j]->dev == dev, EB200_ERR_INVALID, "output %d is null or lives on another device", j);
+        size_t need = (size_t)plan.more_numel[j - 1] * dtype_bytes(plan.more_dtype[j - 1]);
+        EB_REQUIRE(outputs[j]->bytes >= need, EB200_ERR_BOUNDS, "output %d holds %zu bytes, kernel addresses %zu", j, outputs[j]->bytes, need);
+    }
     EB_CHECK_CUDA(cudaSetDevice(dev->index));
     // the output may share storage with a clone: give it its own, keeping the
     // bytes the kernel does not overwrite
@@ -106,6 +111,20 @@ int eb200_kernel_launch(eb200_kernel* k, eb200_buffer* const* inputs, int n_inpu
     for (int i = 0; i < n_inputs; ++i)
         EB_REQUIRE(inputs[i]->storage->ptr != ob->storage->ptr || (optimizer && i == 0), EB200_ERR_INVALID,
                    "input %d aliases the output", i);
+    for (int j = 1; j < n_outputs; ++j) {
+        if ((st = buffer_unshare(outputs[j], true))) return st;
+        for (int i = 0; i < n_inputs; ++i)
+            EB_REQUIRE(inputs[i]->storage->ptr != outputs[j]->storage->ptr, EB200_ERR_INVALID, "input %d aliases output %d", i, j);
+        for (int i = 0; i < j; ++i)
+            EB_REQUIRE(outputs[i]->storage->ptr != outputs[j]->storage->ptr, EB200_ERR_INVALID, "outputs %d and %d are the same buffer", i, j);
+    }
+    if (plan.impl == IMPL_TOKEN_LOGPROB || plan.impl == IMPL_TOKEN_LOGPROB_GRAD || plan.impl == IMPL_DISTILL_TOPK) {
+        const void* in[KMAX_IN];
+        void* outp[KMAX_OUT];
+        for (int i = 0; i < n_inputs; ++i) in[i] = inputs[i]->storage->ptr;
+        for (int j = 0; j < n_outputs; ++j) outp[j] = outputs[j]->storage->ptr;
+        return launch_token(dev, plan, in, outp);
+    }
     // optimizer state (velocity, moments, step counter) is updated in place: give it its own storage first
     if (plan.impl == IMPL_SGD_MOMENTUM || plan.impl == IMPL_ADAM)
         for (int i = 2; i < n_inputs; ++i)

@@ -245,9 +245,107 @@ bool try_gemm(const KParams& p, Plan* plan, int mode) {
 
 }  // namespace
 
+// EB200_K_TOKEN_LOGPROB and EB200_K_DISTILL_TOPK: structured descriptors, shape = {N, V, K}
+static int plan_token(const eb200_kernel_desc* d, int sm_count, Plan* plan) {
+    const bool distill = d->kclass == EB200_K_DISTILL_TOPK, grad = (d->flags & 128) != 0;
+    const char* what = distill ? "distillation" : "token log-probability";
+    EB_REQUIRE(d->ndim == 3, EB200_ERR_INVALID, "%s takes shape {N, V, K}", what);
+    const long long N = d->shape[0], V = d->shape[1], K = d->shape[2];
+    EB_REQUIRE(N >= 0 && V >= 1 && K >= 0, EB200_ERR_INVALID, "%s over [%lld, %lld] with K = %lld", what, N, V, K);
+    EB_REQUIRE(N < (1LL << 27) && V < (1LL << 30), EB200_ERR_UNSUPPORTED, "%s over [%lld, %lld]", what, N, V);
+    EB_REQUIRE((d->flags & ~128) == 0, EB200_ERR_INVALID, "%s has no flags but bit 7", what);
+    EB_REQUIRE(d->scalar >= 1e-30f && d->scalar <= 1e30f, EB200_ERR_INVALID, "%s wants a scale from 1e-30 to 1e30, got %g", what, (double)d->scalar);
+    EB_REQUIRE(d->n_insns == 0 && d->reduce_op == EB200_R_NONE, EB200_ERR_INVALID, "%s carries no map and no reduce", what);
+    int n_in;
+    if (distill) {
+        EB_REQUIRE(K >= 1, EB200_ERR_INVALID, "distillation wants at least one teacher entry per row");
+        EB_REQUIRE(K <= 256, EB200_ERR_UNSUPPORTED, "distillation from %lld teacher entries per row (256 at most)", K);
+        n_in = grad ? 4 : 3;
+        EB_REQUIRE(d->n_inputs == n_in, EB200_ERR_INVALID, "distillation takes %d inputs, got %d", n_in, d->n_inputs);
+    } else {
+        EB_REQUIRE(K <= V && !(grad && K), EB200_ERR_INVALID, grad ? "the token log-probability gradient takes K = 0" : "%lld alternatives of %lld tokens", K, V);
+        EB_REQUIRE(K <= 64, EB200_ERR_UNSUPPORTED, "%lld alternatives per row (64 at most)", K);
+        n_in = d->n_inputs;
+        EB_REQUIRE(grad ? n_in == 4 || n_in == 6 : n_in == 2, EB200_ERR_INVALID,
+                   grad ? "the token log-probability gradient takes 4 inputs, or 6 with the entropy's, got %d" : "token log-probability takes 2 inputs, got %d", n_in);
+    }
+    Plan& pl = *plan;
+    pl = Plan();
+    memset(&pl.p, 0, sizeof(pl.p));
+    TokenShape& t = pl.tok;
+    t.n = N; t.v = (int)V; t.k = (int)K;
+    t.grad = grad;
+    t.entropy = !distill && (!grad || n_in == 6);
+    t.scale = d->scalar;
+    // the role of each input: 0 logits, 1 indices, 2 teacher values, 3 a row vector
+    static const int roles_token[6] = {0, 1, 3, 3, 3, 3}, roles_distill[4] = {0, 2, 1, 3};
+    auto is_float = [](int dt) { return dt == EB200_F32 || dt == EB200_F16 || dt == EB200_BF16; };
+    long long in_bytes = 0;
+    for (int i = 0; i <= n_in; ++i) {
+        const bool out = i == n_in;
+        const eb200_operand& o = out ? d->output : d->inputs[i];
+        const int role = out ? (grad ? 0 : 3) : (distill ? roles_distill[i] : roles_token[i]);
+        EB_REQUIRE(o.n_bounds == 0, EB200_ERR_UNSUPPORTED, "%s operand %d is masked", what, i);
+        EB_REQUIRE(o.offset >= 0 && o.numel >= 0, EB200_ERR_INVALID, "%s operand %d has a negative offset or size", what, i);
+        long long need = N * (distill && (role == 1 || role == 2) ? K : 1);
+        if (role == 0) {
+            EB_REQUIRE(is_float(o.dtype) && (!out || o.dtype == t.dtype), EB200_ERR_UNSUPPORTED, "%s: logits are F32, F16 or BF16, the gradient of the same type", what);
+            const long long pitch = o.strides[0] == 0 ? V : o.strides[0];
+            EB_REQUIRE(pitch >= V && pitch < (1LL << 32) && (o.strides[1] == 1 || o.strides[1] == 0), EB200_ERR_UNSUPPORTED,
+                       "%s operand %d: rows are contiguous and at least %lld elements apart", what, i, V);
+            need = N ? (N - 1) * pitch + V : 0;
+            (out ? t.g_pitch : t.pitch) = pitch;
+            if (!out) t.dtype = o.dtype;
+        } else if (role == 1) {
+            EB_REQUIRE(o.dtype == EB200_I32 || o.dtype == EB200_I64, EB200_ERR_UNSUPPORTED, "%s: token indices are I32 or I64", what);
+            t.id_dtype = o.dtype;
+        } else if (role == 2) {
+            EB_REQUIRE(is_float(o.dtype), EB200_ERR_UNSUPPORTED, "%s: teacher values are F32, F16 or BF16", what);
+            t.teacher_dtype = o.dtype;
+        } else {
+            EB_REQUIRE(o.dtype == EB200_F32, EB200_ERR_UNSUPPORTED, "%s operand %d is F32", what, i);
+        }
+        EB_REQUIRE(o.numel >= need && o.offset <= o.numel - need, EB200_ERR_BOUNDS, "%s operand %d too small", what, i);
+        if (out) {
+            t.g_offset = o.offset;
+        } else {
+            pl.p.in[i].offset = o.offset;
+            pl.in_dtype[i] = o.dtype; pl.in_numel[i] = o.numel; pl.perm[i] = i;
+            in_bytes += (role == 0 ? N * V : need) * dtype_size(o.dtype);
+        }
+    }
+    t.offset = d->inputs[0].offset;
+    pl.n_inputs = n_in;
+    for (int j = 0; j < KMAX_CONSTS; ++j) pl.dyn_input[j] = -1;
+    pl.scalar = d->scalar;
+    pl.out_dtype = EB200_F32;
+    pl.out_numel = d->output.numel;
+    long long out_bytes = 4 * N;
+    if (!distill && grad) {
+        pl.out_dtype = t.dtype;
+        out_bytes = N * V * dtype_size(t.dtype);
+    } else if (distill && grad) {
+        pl.out_numel = N;
+        pl.n_outputs = 2;
+        pl.more_dtype[0] = t.dtype; pl.more_numel[0] = d->output.numel;
+        out_bytes += N * V * dtype_size(t.dtype);
+    } else if (!distill) {
+        pl.n_outputs = K ? 5 : 3;
+        for (int j = 0; j < 4; ++j) { pl.more_dtype[j] = j < 3 ? EB200_F32 : EB200_I32; pl.more_numel[j] = j < 2 ? N : N * K; }
+        out_bytes = 12 * N + 8 * N * K;
+    }
+    pl.algo_bytes = in_bytes + out_bytes;
+    pl.launches = N ? 1 : 0;
+    pl.impl = distill ? IMPL_DISTILL_TOPK : grad ? IMPL_TOKEN_LOGPROB_GRAD : IMPL_TOKEN_LOGPROB;
+    token_variant(&t, sm_count);
+    const char* ty = t.dtype == EB200_F32 ? "f32" : t.dtype == EB200_F16 ? "f16" : "bf16";
+    snprintf(pl.name, sizeof(pl.name), "%s%s_%s%s", distill ? "distill_topk" : "token_logprob", grad ? "_grad" : "", ty, t.lanes ? "_lanes" : t.cluster > 1 ? "_cluster" : "");
+    return EB200_OK;
+}
+
 int build_plan(const eb200_kernel_desc* d, int sm_count, Plan* plan) {
     EB_REQUIRE(d && plan, EB200_ERR_INVALID, "null argument");
-    EB_REQUIRE(d->kclass >= EB200_K_ELEMENTWISE && d->kclass <= EB200_K_MAXPOOL2D, EB200_ERR_INVALID, "unknown kernel class %d", d->kclass);
+    EB_REQUIRE(d->kclass >= EB200_K_ELEMENTWISE && d->kclass <= EB200_K_DISTILL_TOPK, EB200_ERR_INVALID, "unknown kernel class %d", d->kclass);
     if (d->kclass == EB200_K_CONV2D) {
         // structured descriptor: shape = {N, C, H, W, Co, KH, KW, pad}
         EB_REQUIRE(d->ndim == 8, EB200_ERR_INVALID, "conv2d descriptor wants 8 shape entries, got %d", d->ndim);
@@ -306,6 +404,7 @@ int build_plan(const eb200_kernel_desc* d, int sm_count, Plan* plan) {
         else snprintf(pl.name, sizeof(pl.name), "conv2d_igemm_%s%s", c.mode == EB200_GEMM_TF32 ? "tf32" : "3xtf32", c.wgrad ? "_wgrad" : (c.flip ? "_dgrad" : ""));
         return EB200_OK;
     }
+    if (d->kclass == EB200_K_TOKEN_LOGPROB || d->kclass == EB200_K_DISTILL_TOPK) return plan_token(d, sm_count, plan);
     if (d->kclass == EB200_K_MAXPOOL2D) {
         // structured descriptor: shape = {P, H, W, k}; forward x -> y, gradient (g, x, y) -> gx
         const bool grad = (d->flags & 128) != 0;

@@ -1,0 +1,682 @@
+// Log-probabilities of given tokens (entropy, top alternatives), their gradient, and distillation
+// from a teacher's top logits: kernels over [N, V] logits rows, V the vocabulary.
+//
+// With x = scale * z, m = max x, S = sum exp(x - m):
+//   logp = (x_t - m) - ln S,  lse = m + ln S,  H = ln S - (sum e_j (x_j - m)) / S,  e_j = exp(x_j - m)
+// one pass over the row gives m, S and sum e_j (x_j - m).  Every thread keeps them against a
+// reference value of its own (the maximum of the first logits it sees, moved only when a logit
+// exceeds it by more than 2^8 in e_j), so the running maximum costs a comparison per 16 bytes; the
+// partial results are joined against the row's true maximum.  All statistics are f32 whatever the
+// logits' type.  What bounds the pass is DRAM: one exponential, and about six other instructions, per
+// logit against 2 or 4 bytes read.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "common.h"
+
+namespace eb200 {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int TT = 256;                     // threads per CTA
+constexpr int NW = TT / 32;
+constexpr int MAX_CLUSTER = 8;
+constexpr int MAX_K = 64;                   // alternatives
+constexpr int GROUPS = 64;                  // groups of threads whose maxima bound the k-th largest logit, >= MAX_K
+constexpr int CAP = 1024;                   // candidates held at a time
+constexpr int MAX_TEACHER = 256;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr float NEG_INF = -INFINITY;
+constexpr float HEADROOM = 8.f;             // a reference may lie below a logit by this much, in powers of two
+
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <class T> struct Pack { static constexpr int E = 16 / sizeof(T); };   // logits in 16 bytes
+
+__device__ __forceinline__ void unpack(const uint4& u, float (&x)[4], float) {
+    x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y); x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ void unpack(const uint4& u, float (&x)[8], __nv_bfloat16) {
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ void unpack(const uint4& u, float (&x)[8], __half) {
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x; x[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ uint4 pack(const float (&x)[4], float) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+}
+__device__ __forceinline__ uint4 pack(const float (&x)[8], __nv_bfloat16) {
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]); w[i] = *reinterpret_cast<const unsigned*>(&h); }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 pack(const float (&x)[8], __half) {
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]); w[i] = *reinterpret_cast<const unsigned*>(&h); }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ long long load_id(const void* ids, long long i, bool wide) {
+    return wide ? __ldg(reinterpret_cast<const long long*>(ids) + i) : (long long)__ldg(reinterpret_cast<const int*>(ids) + i);
+}
+
+// A row in slots of 16 aligned bytes: slot s holds logits s * E - lead + [0, E).  The first and the last
+// slot may reach over the row's ends; nothing outside the row is ever read.
+template <class T> struct Row {
+    static constexpr int E = Pack<T>::E;
+    const T* p;
+    int v, lead, slots;
+    __device__ Row(const T* row, int v_) : p(row), v(v_) {
+        lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+        slots = (lead + v + E - 1) / E;
+    }
+    __device__ bool whole(int s) const { return s * E >= lead && (s + 1) * E <= lead + v; }
+    __device__ uint4 raw(int s) const { return __ldg(reinterpret_cast<const uint4*>(p - lead) + s); }
+    __device__ void part(int s, float (&x)[E]) const {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int j = s * E - lead + i;
+            x[i] = j >= 0 && j < v ? to_f(__ldg(p + j)) : NEG_INF;
+        }
+    }
+};
+
+// ---- row statistics --------------------------------------------------------------------------------
+
+// Against a reference r: s = sum e, t = sum e * y over y = (z - r) * c, e = 2^y, c = scale * log2(e).
+// mx is the largest logit seen, slot the first slot that holds it (-1: no slot seen).
+struct Acc {
+    float r = NEG_INF, lim = NEG_INF, s = 0.f, t = 0.f, mx = NEG_INF;
+    int slot = -1;
+};
+
+// y of a logit far below its reference counts as -1000: e is 0 there and e * y must not be 0 * inf
+__device__ __forceinline__ float floor_y(float y) { return fmaxf(y, -1000.f); }
+
+__device__ __forceinline__ void move_reference(Acc& a, float r, float c) {
+    const float dy = a.r == NEG_INF ? -1000.f : floor_y((a.r - r) * c);
+    const float f = ex2(dy);
+    a.t = f * (a.t + dy * a.s);
+    a.s *= f;
+    a.r = r;
+    a.lim = r + HEADROOM / c;
+}
+
+template <bool ENT, bool TOP, int E>
+__device__ __forceinline__ void take(Acc& a, const float (&x)[E], int slot, float c) {
+    float mx = x[0];
+#pragma unroll
+    for (int i = 1; i < E; ++i) mx = fmaxf(mx, x[i]);
+    if (mx > a.lim) move_reference(a, mx, c);
+    const float r = a.r == NEG_INF ? 0.f : a.r;      // only -inf so far: e = 0
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const float y = (x[i] - r) * c, e = ex2(y);
+        a.s += e;
+        if (ENT) a.t = fmaf(e, floor_y(y), a.t);
+    }
+    if (TOP) {
+        if (a.slot < 0 || mx > a.mx) a.slot = slot;
+    }
+    a.mx = fmaxf(a.mx, mx);
+}
+
+// this thread's share of a row: slots first, first + step, ...
+template <class T, bool ENT, bool TOP>
+__device__ __forceinline__ void pass(Acc& a, const Row<T>& row, int first, int step, float c) {
+    constexpr int E = Pack<T>::E, U = 4;
+    float x[E];
+    int s = first;
+    if (s < row.slots && !row.whole(s)) { row.part(s, x); take<ENT, TOP>(a, x, s, c); s += step; }
+    const int end = row.whole(row.slots - 1) ? row.slots : row.slots - 1;
+    for (; s + (U - 1) * step < end; s += U * step) {
+        uint4 u[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) u[i] = row.raw(s + i * step);
+#pragma unroll
+        for (int i = 0; i < U; ++i) { unpack(u[i], x, T()); take<ENT, TOP>(a, x, s + i * step, c); }
+    }
+    for (; s < end; s += step) { unpack(row.raw(s), x, T()); take<ENT, TOP>(a, x, s, c); }
+    if (s < row.slots) { row.part(s, x); take<ENT, TOP>(a, x, s, c); }
+}
+
+struct Stat { float r, s, t, mx; };
+
+__device__ __forceinline__ Stat join(const Stat& a, const Stat& b, float c) {
+    Stat o;
+    o.r = fmaxf(a.r, b.r);
+    const float da = a.r == NEG_INF ? -1000.f : floor_y((a.r - o.r) * c), db = b.r == NEG_INF ? -1000.f : floor_y((b.r - o.r) * c);
+    const float fa = ex2(da), fb = ex2(db);
+    o.s = fa * a.s + fb * b.s;
+    o.t = fa * (a.t + da * a.s) + fb * (b.t + db * b.s);
+    o.mx = fmaxf(a.mx, b.mx);
+    return o;
+}
+
+// the row's totals, on every thread of the CTA / cluster, joined in the same order everywhere
+__device__ __forceinline__ Stat totals(const Acc& a, float c, Stat* warp_stat, Stat* cta_stat, int cluster, int rank) {
+    Stat st = {a.r, a.s, a.t, a.mx};
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        Stat q;
+        q.r = __shfl_xor_sync(~0u, st.r, o); q.s = __shfl_xor_sync(~0u, st.s, o);
+        q.t = __shfl_xor_sync(~0u, st.t, o); q.mx = __shfl_xor_sync(~0u, st.mx, o);
+        st = join(st, q, c);
+    }
+    if ((threadIdx.x & 31) == 0) warp_stat[threadIdx.x >> 5] = st;
+    __syncthreads();
+    st = warp_stat[0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) st = join(st, warp_stat[w], c);
+    if (cluster > 1) {
+        cg::cluster_group cl = cg::this_cluster();
+        if ((int)threadIdx.x < cluster) cl.map_shared_rank(cta_stat, threadIdx.x)[rank] = st;
+        cl.sync();
+        st = cta_stat[0];
+        for (int i = 1; i < cluster; ++i) st = join(st, cta_stat[i], c);
+    }
+    return st;
+}
+
+// the statistics against the row's maximum: ln S with S >= 1, and sum e (x - m) / S
+struct Final { float m, s, ln_s, mean; };
+__device__ __forceinline__ Final finish(const Stat& st, float c) {
+    Final f;
+    f.m = st.mx;
+    if (st.mx == NEG_INF && st.s == 0.f) { f.s = 1.f; f.ln_s = 0.f; f.mean = 0.f; return f; }   // only -inf (a NaN makes s NaN)
+    const float dy = (st.r - st.mx) * c, g = ex2(dy);
+    f.s = st.s * g;
+    f.ln_s = logf(f.s);
+    f.mean = LN2 * (st.t / st.s + dy);
+    return f;
+}
+
+// ---- top alternatives ------------------------------------------------------------------------------
+// Order of a logit as an unsigned whole number (NaN like -inf, -0 like 0); 0 is below every logit.
+__device__ __forceinline__ unsigned order_of(float x) {
+    if (x != x) x = NEG_INF;
+    const unsigned b = __float_as_uint(x + 0.f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(unsigned o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+// larger value first, then lower index: unique per logit of a row
+__device__ __forceinline__ unsigned long long key_of(unsigned order, unsigned index) { return (unsigned long long)order << 32 | (0xffffffffu - index); }
+__device__ __forceinline__ unsigned index_of(unsigned long long key) { return 0xffffffffu - (unsigned)key; }
+
+struct TopShared {
+    unsigned long long keys[TT], groups[GROUPS], cand[CAP], peers[MAX_CLUSTER * MAX_K];
+    unsigned long long tau;
+    int owners[TT];
+    int n_owners, n_cand, n_peers[MAX_CLUSTER];
+};
+
+// keeps the k largest of cand[0, n), sorted; all threads; returns how many there are
+__device__ __forceinline__ int keep_largest(TopShared& sh, int n, int k) {
+    constexpr int PER = CAP / TT;
+    unsigned long long mine[PER];
+    int rank[PER];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int at = threadIdx.x + i * TT;
+        rank[i] = CAP;
+        if (at < n) {
+            mine[i] = sh.cand[at];
+            int r = 0;
+            for (int j = 0; j < n; ++j) r += sh.cand[j] > mine[i];
+            rank[i] = r;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (rank[i] < k) sh.cand[rank[i]] = mine[i];
+    __syncthreads();
+    return min(n, k);
+}
+
+// The k largest logits of this CTA's slots (first + tid + i * step) into sh.cand, sorted; returns how many.
+// The k-th largest of 64 group maxima bounds the k-th largest logit from below, so only threads whose
+// maximum reaches it hold candidates; their slots (about 1.3 k threads' worth) are read again, by all threads.
+template <class T>
+__device__ __forceinline__ int top_of_cta(TopShared& sh, const Acc& a, const Row<T>& row, int first, int step, int k) {
+    constexpr int E = Pack<T>::E;
+    const int tid = threadIdx.x;
+    const unsigned long long key = a.slot < 0 ? 0 : key_of(order_of(a.mx), a.slot);
+    sh.keys[tid] = key;
+    if (tid == 0) sh.n_owners = sh.n_cand = 0;
+    __syncthreads();
+    if (tid < GROUPS) {
+        unsigned long long g = 0;
+#pragma unroll
+        for (int i = 0; i < TT / GROUPS; ++i) g = max(g, sh.keys[tid + i * GROUPS]);
+        sh.groups[tid] = g;
+    }
+    __syncthreads();
+    if (tid < GROUPS) {
+        const unsigned long long g = sh.groups[tid];
+        int r = 0;
+#pragma unroll 8
+        for (int j = 0; j < GROUPS; ++j) r += sh.groups[j] > g || (sh.groups[j] == g && j < tid);
+        if (r == k - 1) sh.tau = g;
+    }
+    __syncthreads();
+    const unsigned long long tau = sh.tau;
+    const unsigned tau_order = (unsigned)(tau >> 32);
+    const int tau_slot = (int)(0xffffffffu - (unsigned)tau);       // equal values count up to the end of this slot
+    if (key != 0 && key >= tau) sh.owners[atomicAdd(&sh.n_owners, 1)] = tid;
+    __syncthreads();
+    const int n_own = sh.n_owners, per = (row.slots - first + step - 1) / step;
+    const long long pairs = (long long)n_own * per;
+    auto collect = [&](long long pair) {
+        const int s = first + sh.owners[(int)(pair % n_own)] + (int)(pair / n_own) * step;
+        if (s >= row.slots) return;
+        float x[E];
+        if (row.whole(s)) unpack(row.raw(s), x, T()); else row.part(s, x);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const unsigned o = order_of(x[i]);
+            const int j = s * E - row.lead + i;
+            if (j >= 0 && j < row.v && (tau == 0 || o > tau_order || (o == tau_order && s <= tau_slot))) {
+                const int at = atomicAdd(&sh.n_cand, 1);
+                if (at < CAP) sh.cand[at] = key_of(o, j);
+            }
+        }
+    };
+    for (long long p = tid; p < pairs; p += TT) collect(p);
+    __syncthreads();
+    int n = sh.n_cand;
+    if (n > CAP) {
+        // more than fit (large logits gathered in a few threads' slots): some slots at a time, keeping the k largest
+        constexpr int CHUNK = (CAP - MAX_K) / E / 32 * 32;
+        n = 0;
+        for (long long p0 = 0; p0 < pairs; p0 += CHUNK) {
+            __syncthreads();
+            if (tid == 0) sh.n_cand = n;
+            __syncthreads();
+            const long long p1 = min(p0 + CHUNK, pairs);
+            for (long long p = p0 + tid; p < p1; p += TT) collect(p);
+            __syncthreads();
+            n = keep_largest(sh, sh.n_cand, k);
+        }
+        return n;
+    }
+    return keep_largest(sh, n, k);
+}
+
+// ---- forward ---------------------------------------------------------------------------------------
+
+struct LogprobOut { float *logp, *lse, *entropy, *top; int* top_ids; };
+
+template <class T, bool TOP>
+__global__ void __launch_bounds__(TT, 4) token_logprob_kernel(const T* __restrict__ z, long long pitch, int v, int k, float scale,
+                                                              const void* ids, int wide, LogprobOut out, int cluster) {
+    __shared__ Stat warp_stat[NW], cta_stat[MAX_CLUSTER];
+    extern __shared__ __align__(16) unsigned char dyn[];
+    TopShared& sh = *reinterpret_cast<TopShared*>(dyn);
+    const long long n = blockIdx.x / cluster;
+    const int rank = blockIdx.x % cluster, tid = threadIdx.x;
+    const Row<T> row(z + n * pitch, v);
+    const float c = scale * LOG2E;
+    if (cluster > 1) cg::this_cluster().sync();       // every CTA of the cluster runs before its memory is written
+    float own = NEG_INF;
+    bool there = false;
+    if (rank == 0 && tid == 0) {
+        const long long t = load_id(ids, n, wide);
+        there = t >= 0 && t < v;
+        if (there) own = to_f(row.p[t]);
+    }
+    Acc a;
+    const int first = rank * TT, step = cluster * TT;
+    pass<T, true, TOP>(a, row, first + tid, step, c);
+    const Stat st = totals(a, c, warp_stat, cta_stat, cluster, rank);
+    const Final f = finish(st, c);
+    const bool empty = st.mx == NEG_INF && st.s == 0.f;
+    if (rank == 0 && tid == 0) {
+        out.logp[n] = !there ? 0.f : empty ? NEG_INF : (own - f.m) * scale - f.ln_s;
+        out.lse[n] = f.m * scale + f.ln_s;
+        out.entropy[n] = f.ln_s - f.mean;
+    }
+    if (TOP) {
+        int have = top_of_cta(sh, a, row, first, step, k);
+        if (cluster > 1) {
+            cg::cluster_group cl = cg::this_cluster();
+            TopShared* lead = cl.map_shared_rank(&sh, 0);
+            if (tid < have) lead->peers[rank * MAX_K + tid] = sh.cand[tid];
+            if (tid == 0) lead->n_peers[rank] = have;
+            cl.sync();
+            if (rank != 0) return;
+            __syncthreads();
+            if (tid == 0) sh.n_cand = 0;
+            __syncthreads();
+            for (int i = tid; i < cluster * MAX_K; i += TT)
+                if (i % MAX_K < sh.n_peers[i / MAX_K]) sh.cand[atomicAdd(&sh.n_cand, 1)] = sh.peers[i];
+            __syncthreads();
+            have = keep_largest(sh, sh.n_cand, k);
+        }
+        if (tid < k) {
+            const unsigned long long key = sh.cand[tid];
+            out.top[n * k + tid] = empty ? NEG_INF : (value_of((unsigned)(key >> 32)) - f.m) * scale - f.ln_s;
+            out.top_ids[n * k + tid] = (int)index_of(key);
+        }
+    }
+}
+
+// ---- 16 bytes of logits from any element address ---------------------------------------------------
+
+// bytes [shift, shift + 16) of the 32 bytes (a, b)
+__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int shift) {
+    const unsigned bits = (shift & 3) * 8;
+    unsigned w[5];
+    switch (shift >> 2) {
+        case 0: w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; break;
+        case 1: w[0] = a.y; w[1] = a.z; w[2] = a.w; w[3] = b.x; w[4] = b.y; break;
+        case 2: w[0] = a.z; w[1] = a.w; w[2] = b.x; w[3] = b.y; w[4] = b.z; break;
+        default: w[0] = a.w; w[1] = b.x; w[2] = b.y; w[3] = b.z; w[4] = b.w; break;
+    }
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
+// logits [j, j + E) of a row that starts at p: the aligned 16 bytes around them, as long as those lie inside the row
+template <class T> struct Window {
+    static constexpr int E = Pack<T>::E;
+    uint4 a, b;
+    float x[E];
+    int kind;        // 0 aligned, 1 shifted, 2 element by element
+    __device__ __forceinline__ void load(const T* p, int v, int j, int shift) {
+        const int down = shift / (int)sizeof(T);
+        const uint4* at = reinterpret_cast<const uint4*>(p + j - down);
+        if (shift == 0 && j >= 0 && j + E <= v) { kind = 0; a = __ldg(at); }
+        else if (shift != 0 && j - down >= 0 && j - down + 2 * E <= v) { kind = 1; a = __ldg(at); b = __ldg(at + 1); }
+        else {
+            kind = 2;
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = j + i >= 0 && j + i < v ? to_f(__ldg(p + j + i)) : NEG_INF;
+        }
+    }
+    __device__ __forceinline__ void get(float (&y)[E], int shift) {
+        if (kind == 2) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) y[i] = x[i];
+        } else {
+            unpack(kind == 0 ? a : shifted(a, b, shift), y, T());
+        }
+    }
+};
+
+template <class T> __device__ __forceinline__ void put(T* p, int v, int j, const float (&y)[Pack<T>::E]) {
+    constexpr int E = Pack<T>::E;
+    if (j >= 0 && j + E <= v) {
+        *reinterpret_cast<uint4*>(p + j) = pack(y, T());
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (j + i >= 0 && j + i < v) p[j + i] = from_f<T>(y[i]);
+    }
+}
+
+// ---- gradient --------------------------------------------------------------------------------------
+// d_j = scale * (g_l ([j = t] - p_j) - g_H p_j (ln p_j + H)), p_j = exp(x_j - lse): a stream of logits in and a
+// stream of gradients out, cut along 16-byte slots of the output so that stores stay whole whatever the pitches.
+// A warp takes 32 * GU slots of a row.
+constexpr int GU = 4;
+
+template <class T, bool ENT>
+__global__ void __launch_bounds__(TT) token_logprob_grad_kernel(const T* __restrict__ z, long long pitch, T* __restrict__ g, long long g_pitch, long long rows, int v,
+                                                                float scale, const void* ids, int wide, const float* __restrict__ lse, const float* __restrict__ g_logp,
+                                                                const float* __restrict__ entropy, const float* __restrict__ g_entropy, int per_row) {
+    constexpr int E = Pack<T>::E;
+    const long long task = (long long)blockIdx.x * NW + (threadIdx.x >> 5);
+    const long long n = task / per_row;
+    if (n >= rows) return;
+    const int lane = threadIdx.x & 31, s0 = (int)(task % per_row) * 32 * GU + lane;
+    const T* p = z + n * pitch;
+    T* o = g + n * g_pitch;
+    const int lead = (int)((reinterpret_cast<uintptr_t>(o) & 15) / sizeof(T));
+    const int slots = (lead + v + E - 1) / E;
+    const int shift = (int)(reinterpret_cast<uintptr_t>(p - lead) & 15);
+    const long long t = load_id(ids, n, wide);
+    const float norm = __ldg(lse + n), gl = t >= 0 && t < v ? __ldg(g_logp + n) : 0.f;
+    const float gh = ENT ? __ldg(g_entropy + n) : 0.f, h = ENT ? __ldg(entropy + n) : 0.f;
+    const bool zero = norm == NEG_INF || (gl == 0.f && gh == 0.f);
+    const float up = gl * scale, al = -up, ah = -gh * scale;
+    Window<T> w[GU];
+    if (!zero) {
+#pragma unroll
+        for (int i = 0; i < GU; ++i)
+            if (s0 + i * 32 < slots) w[i].load(p, v, (s0 + i * 32) * E - lead, shift);
+    }
+#pragma unroll
+    for (int i = 0; i < GU; ++i) {
+        const int s = s0 + i * 32, j = s * E - lead;
+        if (s >= slots) break;
+        float x[E];
+        if (zero) {
+#pragma unroll
+            for (int q = 0; q < E; ++q) x[q] = 0.f;
+        } else {
+            w[i].get(x, shift);
+#pragma unroll
+            for (int q = 0; q < E; ++q) {
+                const float d = fmaf(x[q], scale, -norm), pr = ex2(d * LOG2E);
+                x[q] = pr * (ENT ? fmaf(ah, floor_y(d) + h, al) : al);
+            }
+            const long long at = t - j;
+            if (at >= 0 && at < E) {
+#pragma unroll
+                for (int q = 0; q < E; ++q) x[q] += q == (int)at ? up : 0.f;
+            }
+        }
+        put(o, v, j, x);
+    }
+}
+
+// ---- distillation ----------------------------------------------------------------------------------
+// L = sum_k q_k (ln q_k - ln p_{c_k}), q = softmax of the teacher's K values; dL/dz_j = scale * (p_j - sum_{c_k = j} q_k).
+// Warp 0 forms q while the other warps are on the row.  The gradient is the dense scale * weight * p_j first; after a
+// barrier the teacher's places are written again with their q taken off, each from f32 and rounded once.
+struct TeacherShared {
+    float q[MAX_TEACHER], ln_q[MAX_TEACHER], z[MAX_TEACHER];
+    int id[MAX_TEACHER];
+    int some;
+};
+
+template <class T, class U>
+__device__ __forceinline__ void teacher_row(TeacherShared& sh, const T* p, int v, const U* values, const void* ids, int wide, long long n, int k, float c) {
+    constexpr int PER = MAX_TEACHER / 32;
+    const int lane = threadIdx.x & 31;
+    float u[PER], mx = NEG_INF;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int at = lane + i * 32;
+        u[i] = NEG_INF;
+        if (at < k) {
+            const long long id = load_id(ids, n * k + at, wide);
+            const bool there = id >= 0 && id < v;
+            if (there) u[i] = to_f(values[n * k + at]);
+            sh.id[at] = there ? (int)id : -1;
+            sh.z[at] = there ? to_f(__ldg(p + id)) : NEG_INF;
+        }
+        mx = fmaxf(mx, u[i]);
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, o));
+    const float r = mx == NEG_INF ? 0.f : mx;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) { u[i] = (u[i] - r) * c; s += ex2(u[i]); }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    const float ln_s = logf(s);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int at = lane + i * 32;
+        if (at < k) {
+            sh.q[at] = s == 0.f ? 0.f : ex2(u[i]) / s;
+            sh.ln_q[at] = u[i] * LN2 - ln_s;
+        }
+    }
+    if (lane == 0) sh.some = s != 0.f;        // NaN counts
+}
+
+template <class T, class U, bool GRAD>
+__global__ void __launch_bounds__(TT, 4) distill_topk_kernel(const T* __restrict__ z, long long pitch, int v, int k, float scale, const U* __restrict__ values,
+                                                             const void* ids, int wide, const float* __restrict__ weights, float* __restrict__ loss,
+                                                             T* __restrict__ g, long long g_pitch, int cluster) {
+    constexpr int E = Pack<T>::E;
+    __shared__ Stat warp_stat[NW], cta_stat[MAX_CLUSTER];
+    __shared__ TeacherShared sh;
+    const long long n = blockIdx.x / cluster;
+    const int rank = blockIdx.x % cluster, tid = threadIdx.x;
+    const Row<T> row(z + n * pitch, v);
+    const float c = scale * LOG2E;
+    if (cluster > 1) cg::this_cluster().sync();
+    if (tid < 32) teacher_row(sh, row.p, v, values, ids, wide, n, k, c);
+    Acc a;
+    pass<T, false, false>(a, row, rank * TT + tid, cluster * TT, c);
+    const Stat st = totals(a, c, warp_stat, cta_stat, cluster, rank);
+    const Final f = finish(st, c);
+    const bool empty = st.mx == NEG_INF && st.s == 0.f;
+    if (rank == 0 && tid < 32) {
+        float l = 0.f;
+        for (int i = tid; i < k; i += 32) {
+            const float q = sh.q[i], lp = empty ? NEG_INF : (sh.z[i] - f.m) * scale - f.ln_s;
+            if (!(q == 0.f)) l += q * (sh.ln_q[i] - lp);
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+        if (tid == 0) loss[n] = l;
+    }
+    if (!GRAD) return;
+    const float w = __ldg(weights + n);
+    const bool zero = w == 0.f || empty || !sh.some;
+    const float up = w * scale, fac = up / f.s;
+    T* o = g + n * g_pitch;
+    const int lead = (int)((reinterpret_cast<uintptr_t>(o) & 15) / sizeof(T));
+    const int slots = (lead + v + E - 1) / E;
+    const int shift = (int)(reinterpret_cast<uintptr_t>(row.p - lead) & 15);
+    for (int s = rank * TT + tid; s < slots; s += cluster * TT) {
+        const int j = s * E - lead;
+        float x[E];
+        if (zero) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = 0.f;
+        } else {
+            Window<T> win;
+            win.load(row.p, v, j, shift);
+            win.get(x, shift);
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = ex2((x[i] - f.m) * c) * fac;
+        }
+        put(o, v, j, x);
+    }
+    if (zero) return;
+    __syncthreads();
+    if (tid < k) {
+        const int id = sh.id[tid];
+        if (id >= 0 && ((id + lead) / E / TT) % cluster == rank) {
+            float q = 0.f;
+            for (int i = 0; i < k; ++i) q += sh.id[i] == id ? sh.q[i] : 0.f;
+            o[id] = from_f<T>(ex2((sh.z[tid] - f.m) * c) * fac - up * q);
+        }
+    }
+}
+
+// ---- launches --------------------------------------------------------------------------------------
+
+template <class K, class... A>
+int launch_rows(Device* dev, K kernel, long long blocks, int cluster, size_t smem, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(TT);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = dev->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    EB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    count_launch();
+    return EB200_OK;
+}
+
+template <class T>
+int launch_typed(Device* dev, const Plan& plan, const void* const* in, void* const* out) {
+    const TokenShape& t = plan.tok;
+    const T* z = reinterpret_cast<const T*>(in[0]) + t.offset;
+    const int wide = t.id_dtype == EB200_I64, esize = wide ? 8 : 4;
+    auto vec = [&](int i) { return reinterpret_cast<const float*>(in[i]) + plan.p.in[i].offset; };
+    auto index = [&](int i) { return (const void*)(reinterpret_cast<const char*>(in[i]) + plan.p.in[i].offset * esize); };
+    if (plan.impl == IMPL_TOKEN_LOGPROB) {
+        LogprobOut o = {reinterpret_cast<float*>(out[0]) + t.g_offset, reinterpret_cast<float*>(out[1]), reinterpret_cast<float*>(out[2]),
+                        t.k ? reinterpret_cast<float*>(out[3]) : nullptr, t.k ? reinterpret_cast<int*>(out[4]) : nullptr};
+        if (t.k) return launch_rows(dev, token_logprob_kernel<T, true>, t.n * t.cluster, t.cluster, sizeof(TopShared), z, t.pitch, t.v, t.k, t.scale, index(1), wide, o, t.cluster);
+        return launch_rows(dev, token_logprob_kernel<T, false>, t.n * t.cluster, t.cluster, 0, z, t.pitch, t.v, t.k, t.scale, index(1), wide, o, t.cluster);
+    }
+    if (plan.impl == IMPL_TOKEN_LOGPROB_GRAD) {
+        T* g = reinterpret_cast<T*>(out[0]) + t.g_offset;
+        constexpr int E = Pack<T>::E;
+        const int per_row = (t.v + E - 1 + E - 1) / E / (32 * GU) + 1;
+        const long long blocks = (t.n * per_row + NW - 1) / NW;
+        EB_REQUIRE(blocks < (1LL << 31), EB200_ERR_UNSUPPORTED, "token log-probability gradient over %lld rows of %d", t.n, t.v);
+        if (t.entropy) return launch_rows(dev, token_logprob_grad_kernel<T, true>, blocks, 1, 0, z, t.pitch, g, t.g_pitch, t.n, t.v, t.scale, index(1), wide, vec(2), vec(3), vec(4), vec(5), per_row);
+        return launch_rows(dev, token_logprob_grad_kernel<T, false>, blocks, 1, 0, z, t.pitch, g, t.g_pitch, t.n, t.v, t.scale, index(1), wide, vec(2), vec(3), (const float*)nullptr, (const float*)nullptr, per_row);
+    }
+    auto go = [&](auto* values) {
+        using U = std::remove_const_t<std::remove_pointer_t<decltype(values)>>;
+        float* loss = reinterpret_cast<float*>(out[0]) + (t.grad ? 0 : t.g_offset);
+        if (t.grad)
+            return launch_rows(dev, distill_topk_kernel<T, U, true>, t.n * t.cluster, t.cluster, 0, z, t.pitch, t.v, t.k, t.scale, values + plan.p.in[1].offset, index(2), wide, vec(3), loss,
+                               reinterpret_cast<T*>(out[1]) + t.g_offset, t.g_pitch, t.cluster);
+        return launch_rows(dev, distill_topk_kernel<T, U, false>, t.n * t.cluster, t.cluster, 0, z, t.pitch, t.v, t.k, t.scale, values + plan.p.in[1].offset, index(2), wide, (const float*)nullptr, loss,
+                           (T*)nullptr, 0LL, t.cluster);
+    };
+    if (t.teacher_dtype == EB200_F32) return go(reinterpret_cast<const float*>(in[1]));
+    if (t.teacher_dtype == EB200_F16) return go(reinterpret_cast<const __half*>(in[1]));
+    return go(reinterpret_cast<const __nv_bfloat16*>(in[1]));
+}
+
+}  // namespace
+
+// Few rows: the CTAs of a cluster share one, until the GPU is full or a CTA has less than two slots per thread.
+void token_variant(TokenShape* t, int sm_count) {
+    t->cluster = 1;
+    if (t->grad && t->k == 0) return;
+    const long long slots = (long long)t->v / (t->dtype == EB200_F32 ? 4 : 8);
+    while (t->cluster < MAX_CLUSTER && t->n * t->cluster * 2 <= 2LL * sm_count && slots / (t->cluster * 2) >= 2 * TT) t->cluster *= 2;
+}
+
+int launch_token(Device* dev, const Plan& plan, const void* const* in, void* const* out) {
+    if (plan.tok.n == 0) return EB200_OK;
+    switch (plan.tok.dtype) {
+        case EB200_F32: return launch_typed<float>(dev, plan, in, out);
+        case EB200_F16: return launch_typed<__half>(dev, plan, in, out);
+        default: return launch_typed<__nv_bfloat16>(dev, plan, in, out);
+    }
+}
+
+}  // namespace eb200

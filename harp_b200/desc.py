@@ -48,12 +48,13 @@ def bf16_value(bits) -> "np.ndarray":
 
 # eb200_kclass
 K_ELEMENTWISE, K_REDUCE, K_COPY, K_SCATTER, K_SGD, K_CONV2D, K_SCAN, K_SGD_MOMENTUM, K_ADAM, K_SOFTMAX_XENT = 0, 1, 2, 3, 4, 5, 6, 7, 8, 9
-K_MAXPOOL2D = 10
+K_MAXPOOL2D, K_TOKEN_LOGPROB, K_DISTILL_TOPK = 10, 11, 12
 KCLASS_PREFIX = {K_ELEMENTWISE: "E", K_REDUCE: "R", K_COPY: "C", K_SCATTER: "S", K_SGD: "U", K_CONV2D: "CONV",
-                 K_SCAN: "P", K_SGD_MOMENTUM: "UM", K_ADAM: "UA", K_SOFTMAX_XENT: "XENT", K_MAXPOOL2D: "POOL"}
+                 K_SCAN: "P", K_SGD_MOMENTUM: "UM", K_ADAM: "UA", K_SOFTMAX_XENT: "XENT", K_MAXPOOL2D: "POOL", K_TOKEN_LOGPROB: "TLP", K_DISTILL_TOPK: "KD"}
 FLAG_RELU = 64
 FLAG_WFLIP = 128
 FLAG_POOL_GRAD = 128       # K_MAXPOOL2D: the gradient kernel
+FLAG_TOKEN_GRAD = 128      # K_TOKEN_LOGPROB: the gradient kernel; K_DISTILL_TOPK: loss and gradient
 FLAG_WGRAD = 256
 FLAG_NCHW = 512
 FLAG_G_NCHW = 1024
@@ -442,6 +443,46 @@ def softmax_xent(n: int, c: int, scale: float) -> KernelDesc:
     z2 = [0, 0]
     return KernelDesc(K_SOFTMAX_XENT, [n, c], [Operand(z2, 0, F32, n * c), Operand(z2, 0, F32, n * c)],
                       Operand(z2, 0, F32, XENT_GRAD_OFFSET + n * c), None, scalar=scale)
+
+
+def _rows(n: int, v: int, dtype: int, stride: Optional[int], offset: int) -> Operand:
+    """[n, v] rows `stride` elements apart (default v) from element `offset`."""
+    pitch = v if stride is None else stride
+    return Operand([pitch, 1, 0], offset, dtype, offset + ((n - 1) * pitch + v if n else 0))
+
+
+def _dense(count: int, dtype: int = F32) -> Operand:
+    return Operand([0, 0, 0], 0, dtype, count)
+
+
+def token_logprob(n: int, v: int, k: int = 0, dtype: int = F32, ids_dtype: int = I32, scale: float = 1.0,
+                  stride: Optional[int] = None, offset: int = 0) -> KernelDesc:
+    """Log-probabilities of given tokens under softmax(scale * logits) rows, with each row's log-sum-exp,
+    entropy and `k` most likely alternatives.  Inputs: logits [n, v] (rows `stride` elements apart) and
+    tokens [n] (outside [0, v): padding).  Outputs, a buffer each: logp [n], lse [n], entropy [n] and, for
+    k > 0, alternatives' log-probabilities [n, k] and indices [n, k] (I32)."""
+    return KernelDesc(K_TOKEN_LOGPROB, [n, v, k], [_rows(n, v, dtype, stride, offset), _dense(n, ids_dtype)], _dense(n), None, scalar=scale)
+
+
+def token_logprob_grad(n: int, v: int, entropy: bool = False, dtype: int = F32, ids_dtype: int = I32, scale: float = 1.0,
+                       stride: Optional[int] = None, offset: int = 0, grad_stride: Optional[int] = None, grad_offset: int = 0) -> KernelDesc:
+    """Gradient of ``token_logprob`` with respect to the logits.  Inputs: logits, tokens, lse [n], the
+    gradient g_logp [n] and, with `entropy`, the row entropies [n] and the gradient g_entropy [n] of those;
+    output: [n, v] in the logits' type, rows `grad_stride` elements apart."""
+    ins = [_rows(n, v, dtype, stride, offset), _dense(n, ids_dtype), _dense(n), _dense(n)] + ([_dense(n)] * 2 if entropy else [])
+    return KernelDesc(K_TOKEN_LOGPROB, [n, v, 0], ins, _rows(n, v, dtype, grad_stride, grad_offset), None, scalar=scale, flags=FLAG_TOKEN_GRAD)
+
+
+def distill_topk(n: int, v: int, k: int, grad: bool = False, dtype: int = F32, teacher_dtype: int = F32, ids_dtype: int = I32,
+                 scale: float = 1.0, stride: Optional[int] = None, offset: int = 0,
+                 grad_stride: Optional[int] = None, grad_offset: int = 0) -> KernelDesc:
+    """Distillation from a teacher's `k` top logits per row: KL(softmax(scale * teacher values) || softmax(scale
+    * logits) at the teacher's indices).  Inputs: logits [n, v], teacher values [n, k] and indices [n, k] (outside
+    [0, v): no entry); output: loss [n].  With `grad` a fourth input, row weights [n], and a second output: the
+    gradient of sum(weights * loss), [n, v] in the logits' type."""
+    ins = [_rows(n, v, dtype, stride, offset), _dense(n * k, teacher_dtype), _dense(n * k, ids_dtype)] + ([_dense(n)] if grad else [])
+    return KernelDesc(K_DISTILL_TOPK, [n, v, k], ins, _rows(n, v, dtype, grad_stride, grad_offset) if grad else _dense(n), None,
+                      scalar=scale, flags=FLAG_TOKEN_GRAD if grad else 0)
 
 
 def maxpool2d(p: int, h: int, w: int, k: int, relu: bool = False, grad: bool = False) -> KernelDesc:

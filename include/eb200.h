@@ -105,6 +105,35 @@ typedef enum {
                               * equals its window's maximum receives the gradient, the mask-times-gradient of
                               * src/grad/rules.rs:379-399 folded back), 0 elsewhere; with bit 6 also the ReLU's own
                               * gradient mask, gx = x < 0 ? 0 : gx.  All operands contiguous f32 */
+    EB200_K_TOKEN_LOGPROB = 11, /* log-probabilities of given tokens under row softmaxes, with entropy and top alternatives, and
+                              * their gradient (no counterpart in the reference; beside EB200_K_SOFTMAX_XENT, for heads over a
+                              * vocabulary).  shape = {N, V, K}, 0 <= K <= min(V, 64); x = logits * scalar (scalar = 1 /
+                              * temperature, from 1e-30 to 1e30).
+                              * Forward: inputs logits [N, V] (F32 / F16 / BF16) and tokens [N] (I32 / I64); outputs, each a buffer
+                              * of its own: logp [N] = x[t] - lse, lse [N] = ln sum exp x, entropy [N] = -sum p ln p, all F32, and
+                              * for K > 0 the log-probabilities [N, K] F32 and indices [N, K] I32 of the K largest logits, largest
+                              * first, equal ones by the lowest index.  A token outside [0, V) marks padding: its logp is 0, the
+                              * rest of the row's outputs do not depend on it.  -inf logits have probability 0; a row of nothing
+                              * else has logp, lse and alternatives -inf and entropy 0.  A row that holds a NaN or +inf has NaN in
+                              * its float outputs; NaN ranks like -inf among the alternatives.
+                              * Gradient (flags bit 7): inputs logits, tokens, lse [N], g_logp [N] and, with an entropy term,
+                              * entropy [N] and g_entropy [N] (lse and entropy as the forward kernel left them); output [N, V] in
+                              * the logits' type = scalar * (g_logp * ([j = t] - p_j) - g_entropy * p_j * (ln p_j + entropy)), where
+                              * g_logp counts as 0 for a padding token.  A row whose g_logp and g_entropy are 0, and a row whose
+                              * lse is -inf, has gradient 0 whatever its logits; K is 0 */
+    EB200_K_DISTILL_TOPK = 12, /* distillation from a teacher's top logits: shape = {N, V, K}, 1 <= K <= 256; inputs logits [N, V]
+                              * (F32 / F16 / BF16), the teacher's values [N, K] (F32 / F16 / BF16; logits or log-probabilities) and
+                              * their indices [N, K] (I32 / I64).  q = softmax(scalar * values) over the K entries, p = softmax(scalar *
+                              * logits) over all V; output loss [N] F32 = sum_k q_k (ln q_k - ln p[index_k]).  Entries whose
+                              * index is outside [0, V) or whose value is -inf do not take part; a row without entries has loss
+                              * 0 and gradient 0; an index may occur more than once.  Flags bit 7: loss and gradient in one kernel;
+                              * a fourth input, weights [N] F32; outputs loss [N] and the gradient [N, V] (the logits' type) of
+                              * sum_n weight_n * loss_n.  A row of weight 0, and a row of -inf logits, has gradient 0.
+                              * Of both classes: the logits, and the gradient as the descriptor's `output`, may have any row pitch
+                              * >= V (strides[0]; 0 = V), unit column stride and any offset; `output` describes the gradient where
+                              * the kernel writes one (its last output) and output 0 otherwise.  All other operands are dense
+                              * and, except output 0 of a forward kernel and the inputs, start at element 0.  N may be 0.  Results
+                              * do not depend on what else runs: no atomics on memory, one launch, no scratch */
     EB200_K_ADAM = 8         /* Adam::step (crates/nn/src/optim/adam.rs:104-147): inputs p, g, m, v and a one-element
                               * I32 step counter t; the output receives p; m, v and t are updated IN PLACE (t <- t + 1
                               * on the device, so a captured step can be replayed); scalar = lr, hyper[0..2] = beta1,
