@@ -498,14 +498,24 @@ __global__ void __launch_bounds__(TT) token_logprob_grad_kernel(const T* __restr
 // L = sum_k q_k (ln q_k - ln p_{c_k}), q = softmax of the teacher's K values; dL/dz_j = scale * (p_j - sum_{c_k = j} q_k).
 // Warp 0 forms q while the other warps are on the row.  The gradient is the dense scale * weight * p_j first; after a
 // barrier the teacher's places are written again with their q taken off, each from f32 and rounded once.
+struct Teacher {
+    const void *values, *ids;
+    int dtype, wide;
+    __device__ __forceinline__ float value(long long i) const {
+        if (dtype == EB200_F32) return __ldg(reinterpret_cast<const float*>(values) + i);
+        if (dtype == EB200_F16) return to_f(__ldg(reinterpret_cast<const __half*>(values) + i));
+        return to_f(__ldg(reinterpret_cast<const __nv_bfloat16*>(values) + i));
+    }
+};
+
 struct TeacherShared {
     float q[MAX_TEACHER], ln_q[MAX_TEACHER], z[MAX_TEACHER];
     int id[MAX_TEACHER];
     int some;
 };
 
-template <class T, class U>
-__device__ __forceinline__ void teacher_row(TeacherShared& sh, const T* p, int v, const U* values, const void* ids, int wide, long long n, int k, float c) {
+template <class T>
+__device__ __forceinline__ void teacher_row(TeacherShared& sh, const T* p, int v, const Teacher& te, long long n, int k, float c) {
     constexpr int PER = MAX_TEACHER / 32;
     const int lane = threadIdx.x & 31;
     float u[PER], mx = NEG_INF;
@@ -514,9 +524,9 @@ __device__ __forceinline__ void teacher_row(TeacherShared& sh, const T* p, int v
         const int at = lane + i * 32;
         u[i] = NEG_INF;
         if (at < k) {
-            const long long id = load_id(ids, n * k + at, wide);
+            const long long id = load_id(te.ids, n * k + at, te.wide);
             const bool there = id >= 0 && id < v;
-            if (there) u[i] = to_f(values[n * k + at]);
+            if (there) u[i] = te.value(n * k + at);
             sh.id[at] = there ? (int)id : -1;
             sh.z[at] = there ? to_f(__ldg(p + id)) : NEG_INF;
         }
@@ -542,9 +552,8 @@ __device__ __forceinline__ void teacher_row(TeacherShared& sh, const T* p, int v
     if (lane == 0) sh.some = s != 0.f;        // NaN counts
 }
 
-template <class T, class U, bool GRAD>
-__global__ void __launch_bounds__(TT, 4) distill_topk_kernel(const T* __restrict__ z, long long pitch, int v, int k, float scale, const U* __restrict__ values,
-                                                             const void* ids, int wide, const float* __restrict__ weights, float* __restrict__ loss,
+template <class T, bool GRAD>
+__global__ void __launch_bounds__(TT, 4) distill_topk_kernel(const T* __restrict__ z, long long pitch, int v, int k, float scale, Teacher te, const float* __restrict__ weights, float* __restrict__ loss,
                                                              T* __restrict__ g, long long g_pitch, int cluster) {
     constexpr int E = Pack<T>::E;
     __shared__ Stat warp_stat[NW], cta_stat[MAX_CLUSTER];
@@ -554,7 +563,7 @@ __global__ void __launch_bounds__(TT, 4) distill_topk_kernel(const T* __restrict
     const Row<T> row(z + n * pitch, v);
     const float c = scale * LOG2E;
     if (cluster > 1) cg::this_cluster().sync();
-    if (tid < 32) teacher_row(sh, row.p, v, values, ids, wide, n, k, c);
+    if (tid < 32) teacher_row(sh, row.p, v, te, n, k, c);
     Acc a;
     pass<T, false, false>(a, row, rank * TT + tid, cluster * TT, c);
     const Stat st = totals(a, c, warp_stat, cta_stat, cluster, rank);
@@ -605,6 +614,175 @@ __global__ void __launch_bounds__(TT, 4) distill_topk_kernel(const T* __restrict
     }
 }
 
+// ---- short rows ------------------------------------------------------------------------------------
+// A row of at most L * E logits lies in the registers of L lanes (logit j in lane j % L), so its maximum is known
+// before the first exponential and S is 1 + the others' sum: ln S = log1p keeps its digits on confident rows.
+// 65536 rows of 10: L = 4 lanes a row, 64 rows a CTA.
+enum { LANES_LOGPROB, LANES_GRAD, LANES_DISTILL, LANES_DISTILL_GRAD };
+
+struct LanesArgs {
+    const void* z;
+    void* g;
+    long long pitch, g_pitch, rows;
+    int v, k;
+    float scale;
+    const void* ids;
+    int wide;
+    LogprobOut out;                                        // logprob
+    const float *lse, *g_logp, *entropy, *g_entropy;       // its gradient
+    Teacher te;                                            // distillation
+    const float* weights;
+    float* loss;
+};
+
+template <int L> __device__ __forceinline__ float lanes_max(float x) {
+#pragma unroll
+    for (int o = L / 2; o >= 1; o >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
+    return x;
+}
+template <int L> __device__ __forceinline__ float lanes_sum(float x) {
+#pragma unroll
+    for (int o = L / 2; o >= 1; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+    return x;
+}
+
+template <class T, int L, int E, int MODE>
+__global__ void __launch_bounds__(TT) token_lanes_kernel(LanesArgs a) {
+    extern __shared__ __align__(16) unsigned char dyn[];
+    const long long want = ((long long)blockIdx.x * TT + threadIdx.x) / L;
+    const bool live = want < a.rows;
+    const long long n = live ? want : a.rows - 1;          // lanes without a row follow the last one and store nothing
+    const int lane = threadIdx.x % L;
+    const T* p = reinterpret_cast<const T*>(a.z) + n * a.pitch;
+    const float c = a.scale * LOG2E;
+    float x[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = lane + i * L < a.v ? to_f(__ldg(p + lane + i * L)) : NEG_INF;
+
+    if (MODE == LANES_GRAD) {
+        const long long t = load_id(a.ids, n, a.wide);
+        const float norm = __ldg(a.lse + n), gl = t >= 0 && t < a.v ? __ldg(a.g_logp + n) : 0.f;
+        const float gh = a.g_entropy ? __ldg(a.g_entropy + n) : 0.f, h = a.g_entropy ? __ldg(a.entropy + n) : 0.f;
+        const bool zero = norm == NEG_INF || (gl == 0.f && gh == 0.f);
+        T* g = reinterpret_cast<T*>(a.g) + n * a.g_pitch;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int j = lane + i * L;
+            if (live && j < a.v) {
+                const float d = fmaf(x[i], a.scale, -norm), pr = ex2(d * LOG2E);
+                float r = -a.scale * pr * fmaf(gh, floor_y(d) + h, gl);
+                if (j == t) r += gl * a.scale;
+                g[j] = from_f<T>(zero ? 0.f : r);
+            }
+        }
+        return;
+    }
+
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < E; ++i) m = fmaxf(m, x[i]);
+    m = lanes_max<L>(fmaxf(m, NEG_INF));
+    unsigned top = ~0u;                                    // the maximum's place, the lowest of equal ones
+#pragma unroll
+    for (int i = E - 1; i >= 0; --i)
+        if (x[i] == m && lane + i * L < a.v) top = lane + i * L;
+#pragma unroll
+    for (int o = L / 2; o >= 1; o >>= 1) top = min(top, __shfl_xor_sync(~0u, top, o));
+    const float ref = m == NEG_INF ? 0.f : m;
+    float others = 0.f, sum_y = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const float y = (x[i] - ref) * c, e = ex2(y);
+        if (lane + i * L != (int)top) {
+            others += e;
+            if (MODE == LANES_LOGPROB) sum_y = fmaf(e, floor_y(y), sum_y);
+        }
+    }
+    others = lanes_sum<L>(others);
+    if (m == INFINITY) others = NAN;
+    const bool empty = m == NEG_INF && others == 0.f;
+    const float ln_s = empty ? 0.f : log1pf(others), inv_s = 1.f / (1.f + others);
+
+    if (MODE == LANES_LOGPROB) {
+        sum_y = lanes_sum<L>(sum_y);
+        if (live && lane == 0) {
+            const long long t = load_id(a.ids, n, a.wide);
+            const bool there = t >= 0 && t < a.v;
+            a.out.logp[n] = !there ? 0.f : empty ? NEG_INF : (to_f(__ldg(p + t)) - m) * a.scale - ln_s;
+            a.out.lse[n] = m * a.scale + ln_s;
+            a.out.entropy[n] = empty ? 0.f : ln_s - LN2 * sum_y * inv_s;
+        }
+        unsigned taken = 0;
+        for (int r = 0; r < a.k; ++r) {
+            unsigned best = 0, at = ~0u;                   // orders of logits are above 0
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const unsigned o = lane + i * L < a.v && !(taken >> i & 1) ? order_of(x[i]) : 0;
+                if (o > best) { best = o; at = lane + i * L; }
+            }
+            unsigned long long key = best ? key_of(best, at) : 0;
+#pragma unroll
+            for (int o = L / 2; o >= 1; o >>= 1) key = max(key, __shfl_xor_sync(~0u, key, o));
+            const unsigned j = index_of(key);
+            if (j % L == (unsigned)lane) taken |= 1u << (j / L);
+            if (live && lane == r % L) {
+                a.out.top[n * a.k + r] = empty ? NEG_INF : (value_of((unsigned)(key >> 32)) - m) * a.scale - ln_s;
+                a.out.top_ids[n * a.k + r] = (int)j;
+            }
+        }
+        return;
+    }
+
+    // distillation: the teacher's entries of this row in shared memory
+    float* q = reinterpret_cast<float*>(dyn) + (long long)(threadIdx.x / L) * 3 * a.k;
+    float* zk = q + a.k;
+    int* id = reinterpret_cast<int*>(zk + a.k);
+    float mu = NEG_INF;
+    for (int i = lane; i < a.k; i += L) {
+        const long long t = load_id(a.te.ids, n * a.k + i, a.te.wide);
+        const bool there = t >= 0 && t < a.v;
+        const float u = there ? a.te.value(n * a.k + i) : NEG_INF;
+        q[i] = u;
+        id[i] = there ? (int)t : -1;
+        zk[i] = there ? to_f(__ldg(p + t)) : NEG_INF;
+        mu = fmaxf(mu, u);
+    }
+    mu = lanes_max<L>(mu);
+    if (mu == NEG_INF) mu = 0.f;
+    float total = 0.f;
+    for (int i = lane; i < a.k; i += L) total += ex2((q[i] - mu) * c);
+    total = lanes_sum<L>(total);
+    const bool some = total != 0.f;
+    const float ln_total = logf(total);
+    float loss = 0.f;
+    for (int i = lane; i < a.k; i += L) {
+        const float y = (q[i] - mu) * c, qi = some ? ex2(y) / total : 0.f;
+        const float lp = empty ? NEG_INF : (zk[i] - m) * a.scale - ln_s;
+        if (!(qi == 0.f)) loss += qi * ((y * LN2 - ln_total) - lp);
+        q[i] = qi;
+    }
+    loss = lanes_sum<L>(loss);
+    if (live && lane == 0) a.loss[n] = loss;
+    if (MODE != LANES_DISTILL_GRAD) return;
+    const float w = __ldg(a.weights + n);
+    const bool zero = w == 0.f || empty || !some;
+    const float up = w * a.scale, fac = up * inv_s;
+    T* g = reinterpret_cast<T*>(a.g) + n * a.g_pitch;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int j = lane + i * L;
+        if (live && j < a.v) g[j] = from_f<T>(zero ? 0.f : ex2((x[i] - ref) * c) * fac);
+    }
+    __syncwarp();                                          // q and id of all lanes; the places below are written again
+    if (zero || !live) return;
+    for (int i = lane; i < a.k; i += L) {
+        if (id[i] < 0) continue;
+        float sum = 0.f;
+        for (int h = 0; h < a.k; ++h) sum += id[h] == id[i] ? q[h] : 0.f;
+        g[id[i]] = from_f<T>(ex2((zk[i] - ref) * c) * fac - up * sum);
+    }
+}
+
 // ---- launches --------------------------------------------------------------------------------------
 
 template <class K, class... A>
@@ -624,9 +802,53 @@ int launch_rows(Device* dev, K kernel, long long blocks, int cluster, size_t sme
     return EB200_OK;
 }
 
+template <class T, int L, int E>
+int launch_lanes_of(Device* dev, const Plan& plan, const LanesArgs& a, size_t smem) {
+    const long long blocks = (a.rows + TT / L - 1) / (TT / L);
+    switch (plan.impl) {
+        case IMPL_TOKEN_LOGPROB: return launch_rows(dev, token_lanes_kernel<T, L, E, LANES_LOGPROB>, blocks, 1, 0, a);
+        case IMPL_TOKEN_LOGPROB_GRAD: return launch_rows(dev, token_lanes_kernel<T, L, E, LANES_GRAD>, blocks, 1, 0, a);
+        default: break;
+    }
+    if (plan.tok.grad) return launch_rows(dev, token_lanes_kernel<T, L, E, LANES_DISTILL_GRAD>, blocks, 1, smem, a);
+    return launch_rows(dev, token_lanes_kernel<T, L, E, LANES_DISTILL>, blocks, 1, smem, a);
+}
+
+template <class T>
+int launch_lanes(Device* dev, const Plan& plan, const void* const* in, void* const* out) {
+    const TokenShape& t = plan.tok;
+    const int wide = t.id_dtype == EB200_I64, esize = wide ? 8 : 4;
+    auto vec = [&](int i) { return reinterpret_cast<const float*>(in[i]) + plan.p.in[i].offset; };
+    auto index = [&](int i) { return (const void*)(reinterpret_cast<const char*>(in[i]) + plan.p.in[i].offset * esize); };
+    LanesArgs a = {};
+    a.z = reinterpret_cast<const T*>(in[0]) + t.offset;
+    a.pitch = t.pitch; a.g_pitch = t.g_pitch; a.rows = t.n; a.v = t.v; a.k = t.k; a.scale = t.scale; a.wide = wide;
+    if (plan.impl == IMPL_DISTILL_TOPK) {
+        a.te = {reinterpret_cast<const char*>(in[1]) + plan.p.in[1].offset * (t.teacher_dtype == EB200_F32 ? 4 : 2), index(2), t.teacher_dtype, wide};
+        a.loss = reinterpret_cast<float*>(out[0]) + (t.grad ? 0 : t.g_offset);
+        if (t.grad) { a.weights = vec(3); a.g = reinterpret_cast<T*>(out[1]) + t.g_offset; }
+    } else {
+        a.ids = index(1);
+        if (t.grad) {
+            a.lse = vec(2); a.g_logp = vec(3);
+            if (t.entropy) { a.entropy = vec(4); a.g_entropy = vec(5); }
+            a.g = reinterpret_cast<T*>(out[0]) + t.g_offset;
+        } else {
+            a.out = {reinterpret_cast<float*>(out[0]) + t.g_offset, reinterpret_cast<float*>(out[1]), reinterpret_cast<float*>(out[2]),
+                     t.k ? reinterpret_cast<float*>(out[3]) : nullptr, t.k ? reinterpret_cast<int*>(out[4]) : nullptr};
+        }
+    }
+    const size_t smem = (size_t)(TT / t.lanes) * t.k * 12;
+    if (t.lanes == 4) return launch_lanes_of<T, 4, 4>(dev, plan, a, smem);
+    if (t.lanes == 8) return launch_lanes_of<T, 8, 8>(dev, plan, a, smem);
+    if (t.v <= 256) return launch_lanes_of<T, 32, 8>(dev, plan, a, smem);
+    return launch_lanes_of<T, 32, 32>(dev, plan, a, smem);
+}
+
 template <class T>
 int launch_typed(Device* dev, const Plan& plan, const void* const* in, void* const* out) {
     const TokenShape& t = plan.tok;
+    if (t.lanes) return launch_lanes<T>(dev, plan, in, out);
     const T* z = reinterpret_cast<const T*>(in[0]) + t.offset;
     const int wide = t.id_dtype == EB200_I64, esize = wide ? 8 : 4;
     auto vec = [&](int i) { return reinterpret_cast<const float*>(in[i]) + plan.p.in[i].offset; };
@@ -646,26 +868,30 @@ int launch_typed(Device* dev, const Plan& plan, const void* const* in, void* con
         if (t.entropy) return launch_rows(dev, token_logprob_grad_kernel<T, true>, blocks, 1, 0, z, t.pitch, g, t.g_pitch, t.n, t.v, t.scale, index(1), wide, vec(2), vec(3), vec(4), vec(5), per_row);
         return launch_rows(dev, token_logprob_grad_kernel<T, false>, blocks, 1, 0, z, t.pitch, g, t.g_pitch, t.n, t.v, t.scale, index(1), wide, vec(2), vec(3), (const float*)nullptr, (const float*)nullptr, per_row);
     }
-    auto go = [&](auto* values) {
-        using U = std::remove_const_t<std::remove_pointer_t<decltype(values)>>;
-        float* loss = reinterpret_cast<float*>(out[0]) + (t.grad ? 0 : t.g_offset);
-        if (t.grad)
-            return launch_rows(dev, distill_topk_kernel<T, U, true>, t.n * t.cluster, t.cluster, 0, z, t.pitch, t.v, t.k, t.scale, values + plan.p.in[1].offset, index(2), wide, vec(3), loss,
-                               reinterpret_cast<T*>(out[1]) + t.g_offset, t.g_pitch, t.cluster);
-        return launch_rows(dev, distill_topk_kernel<T, U, false>, t.n * t.cluster, t.cluster, 0, z, t.pitch, t.v, t.k, t.scale, values + plan.p.in[1].offset, index(2), wide, (const float*)nullptr, loss,
-                           (T*)nullptr, 0LL, t.cluster);
-    };
-    if (t.teacher_dtype == EB200_F32) return go(reinterpret_cast<const float*>(in[1]));
-    if (t.teacher_dtype == EB200_F16) return go(reinterpret_cast<const __half*>(in[1]));
-    return go(reinterpret_cast<const __nv_bfloat16*>(in[1]));
+    const int vsize = t.teacher_dtype == EB200_F32 ? 4 : 2;
+    const Teacher te = {reinterpret_cast<const char*>(in[1]) + plan.p.in[1].offset * vsize, index(2), t.teacher_dtype, wide};
+    float* loss = reinterpret_cast<float*>(out[0]) + (t.grad ? 0 : t.g_offset);
+    if (t.grad)
+        return launch_rows(dev, distill_topk_kernel<T, true>, t.n * t.cluster, t.cluster, 0, z, t.pitch, t.v, t.k, t.scale, te, vec(3), loss,
+                           reinterpret_cast<T*>(out[1]) + t.g_offset, t.g_pitch, t.cluster);
+    return launch_rows(dev, distill_topk_kernel<T, false>, t.n * t.cluster, t.cluster, 0, z, t.pitch, t.v, t.k, t.scale, te, (const float*)nullptr, loss, (T*)nullptr, 0LL, t.cluster);
 }
 
 }  // namespace
 
-// Few rows: the CTAs of a cluster share one, until the GPU is full or a CTA has less than two slots per thread.
+// Short rows in registers: 4 lanes up to 16 logits, 8 up to 64, a warp up to 256 (the gradient) or 1024 (the rest).
+// A distillation's teacher entries lie in shared memory, so many entries per row want more lanes.
+// Few longer rows: the CTAs of a cluster share one, until the GPU is full or a CTA has less than two slots per thread.
 void token_variant(TokenShape* t, int sm_count) {
     t->cluster = 1;
-    if (t->grad && t->k == 0) return;
+    t->lanes = 0;
+    const bool logprob_grad = t->grad && t->k == 0;
+    if (t->v <= (logprob_grad ? 256 : 1024)) {
+        t->lanes = t->v <= 16 ? 4 : t->v <= 64 ? 8 : 32;
+        while (t->lanes < 32 && TT / t->lanes * t->k * 12 > 32768) t->lanes = t->lanes == 4 ? 8 : 32;
+        return;
+    }
+    if (logprob_grad) return;
     const long long slots = (long long)t->v / (t->dtype == EB200_F32 ? 4 : 8);
     while (t->cluster < MAX_CLUSTER && t->n * t->cluster * 2 <= 2LL * sm_count && slots / (t->cluster * 2) >= 2 * TT) t->cluster *= 2;
 }
