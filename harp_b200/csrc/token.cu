@@ -3,17 +3,14 @@
 //
 // With x = scale * z, m = max x, S = sum exp(x - m):
 //   logp = (x_t - m) - ln S,  lse = m + ln S,  H = ln S - (sum e_j (x_j - m)) / S,  e_j = exp(x_j - m)
-// one pass over the row gives m, S and sum e_j (x_j - m).  Every thread keeps them against a
-// reference value of its own (the maximum of the first logits it sees, moved only when a logit
-// exceeds it by more than 2^8 in e_j), so the running maximum costs a comparison per 16 bytes; the
-// partial results are joined against the row's true maximum.  All statistics are f32 whatever the
-// logits' type.  What bounds the pass is DRAM: one exponential, and about six other instructions, per
-// logit against 2 or 4 bytes read.
+// one pass over the row gives m, S and sum e_j (x_j - m).  All statistics are f32 whatever the logits' type.  What
+// bounds the pass is DRAM: one exponential, and about five other instructions, per logit against 2 or 4 bytes read.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -106,112 +103,244 @@ template <class T> struct Row {
 
 // ---- row statistics --------------------------------------------------------------------------------
 
-// Against a reference r: s = sum e, t = sum e * y over y = (z - r) * c, e = 2^y, c = scale * log2(e).
-// mx is the largest logit seen, slot the first slot that holds it (-1: no slot seen).
+// A thread's sums are held against a reference 2^rc of its own, rc a whole number, so that moving or joining
+// references scales by powers of two: s = sum e, t = sum e * y over y = x * c - rc (one rounding), e = 2^y,
+// c = scale * log2(e).  rc is set by the first logits and moves when y would exceed HEADROOM.  mx is the largest
+// logit seen, slot the first slot that holds it (-1: no slot seen).  Logits below -FAR / c (masks) never set a
+// reference and count as 0; a row whose maximum lies beyond NEAR / c is summed again against that maximum.
+constexpr float NEAR = 4194304.f, FAR = 8388608.f;
+
 struct Acc {
-    float r = NEG_INF, lim = NEG_INF, s = 0.f, t = 0.f, mx = NEG_INF;
+    float rc = 0.f, lim, mx = NEG_INF;
+    float2 s = {0.f, 0.f}, t = {0.f, 0.f};
     int slot = -1;
+    __device__ __forceinline__ explicit Acc(float c) : lim(-FAR / c) {}
 };
 
 // y of a logit far below its reference counts as -1000: e is 0 there and e * y must not be 0 * inf
 __device__ __forceinline__ float floor_y(float y) { return fmaxf(y, -1000.f); }
 
-__device__ __forceinline__ void move_reference(Acc& a, float r, float c) {
-    const float dy = a.r == NEG_INF ? -1000.f : floor_y((a.r - r) * c);
-    const float f = ex2(dy);
-    a.t = f * (a.t + dy * a.s);
-    a.s *= f;
-    a.r = r;
-    a.lim = r + HEADROOM / c;
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{ .reg .b64 a, b, c, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7}; fma.rn.f32x2 d, a, b, c; mov.b64 {%0, %1}, d; }"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{ .reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; add.rn.f32x2 d, a, b; mov.b64 {%0, %1}, d; }"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
 }
 
-template <bool ENT, bool TOP, int E>
-__device__ __forceinline__ void take(Acc& a, const float (&x)[E], int slot, float c) {
-    float mx = x[0];
+__device__ __forceinline__ void move_reference(Acc& a, float mx, float c) {
+    const float rc = fminf(rintf(mx * c), FAR);
+    const float dy = fminf(floor_y(a.rc - rc), 0.f), f = ex2(dy);       // 0 sums before the first reference
+    a.t.x = f * fmaf(dy, a.s.x, a.t.x); a.t.y = f * fmaf(dy, a.s.y, a.t.y);
+    a.s.x *= f; a.s.y *= f;
+    a.rc = rc;
+    a.lim = (rc + HEADROOM) / c;
+}
+
+// 16 bytes of logits as they lie in memory: their maximum (NaN left out), and pairs of them in f32.  With an entropy,
+// -inf becomes a finite value whose e is 0 (`low`; NaN stays).
+template <class T> struct Bits;
+template <> struct Bits<float> {
+    static __device__ __forceinline__ float largest(const uint4& u) {
+        return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    }
+    template <bool ENT> static __device__ __forceinline__ void pairs(const uint4& u, float2 (&x)[2], float c) {
+        x[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+        x[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+        if (ENT) {
+            const float low = fmaxf(-2.f * FAR / c, -3.402823466e38f);
 #pragma unroll
-    for (int i = 1; i < E; ++i) mx = fmaxf(mx, x[i]);
+            for (int i = 0; i < 2; ++i) { x[i].x = x[i].x < low ? low : x[i].x; x[i].y = x[i].y < low ? low : x[i].y; }
+        }
+    }
+};
+template <> struct Bits<__nv_bfloat16> {
+    static __device__ __forceinline__ __nv_bfloat162 as(unsigned w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
+    static __device__ __forceinline__ float largest(const uint4& u) {
+        const __nv_bfloat162 m = __hmax2(__hmax2(as(u.x), as(u.y)), __hmax2(as(u.z), as(u.w)));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+    template <bool ENT> static __device__ __forceinline__ void pairs(const uint4& u, float2 (&x)[4], float c) {
+        unsigned w[4] = {u.x, u.y, u.z, u.w};
+        const __nv_bfloat162 low = __float2bfloat162_rn(fmaxf(-2.f * FAR / c, -3.3e38f));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (ENT) { const __nv_bfloat162 h = __hmax2_nan(as(w[i]), low); w[i] = *reinterpret_cast<const unsigned*>(&h); }
+            x[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+        }
+    }
+};
+template <> struct Bits<__half> {
+    static __device__ __forceinline__ __half2 as(unsigned w) { return *reinterpret_cast<__half2*>(&w); }
+    static __device__ __forceinline__ float largest(const uint4& u) {
+        const __half2 m = __hmax2(__hmax2(as(u.x), as(u.y)), __hmax2(as(u.z), as(u.w)));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+    template <bool ENT> static __device__ __forceinline__ void pairs(const uint4& u, float2 (&x)[4], float) {
+        const unsigned w[4] = {u.x, u.y, u.z, u.w};
+        const __half2 low = __float2half2_rn(-65504.f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __half22float2(ENT ? __hmax2_nan(as(w[i]), low) : as(w[i]));
+    }
+};
+
+template <bool ENT>
+__device__ __forceinline__ void add_pair(Acc& a, float2 x, float c) {
+    const float2 y = fma2(x, make_float2(c, c), make_float2(-a.rc, -a.rc));
+    const float2 e = make_float2(ex2(y.x), ex2(y.y));
+    a.s = add2(a.s, e);
+    if (ENT) a.t = fma2(e, y, a.t);
+}
+
+// N slots of a thread: one comparison against the reference for all of them
+template <class T, bool ENT, bool TOP, int N>
+__device__ __forceinline__ void take(Acc& a, const uint4 (&u)[N], int slot, int step, float c) {
+    float mx = NEG_INF;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float m = Bits<T>::largest(u[i]);
+        if (TOP) {
+            if (m > a.mx) { a.mx = m; a.slot = slot + i * step; }
+        }
+        mx = fmaxf(mx, m);
+    }
+    if (!TOP) a.mx = fmaxf(a.mx, mx);
     if (mx > a.lim) move_reference(a, mx, c);
-    const float r = a.r == NEG_INF ? 0.f : a.r;      // only -inf so far: e = 0
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const float y = (x[i] - r) * c, e = ex2(y);
-        a.s += e;
-        if (ENT) a.t = fmaf(e, floor_y(y), a.t);
+    for (int i = 0; i < N; ++i) {
+        float2 x[Pack<T>::E / 2];
+        Bits<T>::template pairs<ENT>(u[i], x, c);
+#pragma unroll
+        for (int q = 0; q < Pack<T>::E / 2; ++q) add_pair<ENT>(a, x[q], c);
     }
-    if (TOP) {
-        if (a.slot < 0 || mx > a.mx) a.slot = slot;
-    }
+}
+
+// a slot that reaches over the row's ends (its places outside hold -inf)
+template <class T, bool ENT, bool TOP>
+__device__ __forceinline__ void take_part(Acc& a, const Row<T>& row, int slot, float c) {
+    float x[Pack<T>::E], mx = NEG_INF;
+    row.part(slot, x);
+#pragma unroll
+    for (int i = 0; i < Pack<T>::E; ++i) mx = fmaxf(mx, x[i]);
+    if (TOP && mx > a.mx) a.slot = slot;
     a.mx = fmaxf(a.mx, mx);
+    if (mx > a.lim) move_reference(a, mx, c);
+#pragma unroll
+    for (int i = 0; i < Pack<T>::E; ++i) {
+        const float y = fmaf(x[i], c, -a.rc), e = ex2(y);
+        a.s.x += e;
+        if (ENT) a.t.x = fmaf(e, floor_y(y), a.t.x);
+    }
 }
 
 // this thread's share of a row: slots first, first + step, ...
 template <class T, bool ENT, bool TOP>
 __device__ __forceinline__ void pass(Acc& a, const Row<T>& row, int first, int step, float c) {
-    constexpr int E = Pack<T>::E, U = 4;
-    float x[E];
+    constexpr int U = 4;
     int s = first;
-    if (s < row.slots && !row.whole(s)) { row.part(s, x); take<ENT, TOP>(a, x, s, c); s += step; }
+    if (s < row.slots) a.slot = s;
+    if (s < row.slots && !row.whole(s)) { take_part<T, ENT, TOP>(a, row, s, c); s += step; }
     const int end = row.whole(row.slots - 1) ? row.slots : row.slots - 1;
     for (; s + (U - 1) * step < end; s += U * step) {
         uint4 u[U];
 #pragma unroll
         for (int i = 0; i < U; ++i) u[i] = row.raw(s + i * step);
-#pragma unroll
-        for (int i = 0; i < U; ++i) { unpack(u[i], x, T()); take<ENT, TOP>(a, x, s + i * step, c); }
+        take<T, ENT, TOP>(a, u, s, step, c);
     }
-    for (; s < end; s += step) { unpack(row.raw(s), x, T()); take<ENT, TOP>(a, x, s, c); }
-    if (s < row.slots) { row.part(s, x); take<ENT, TOP>(a, x, s, c); }
+    for (; s < end; s += step) {
+        const uint4 u[1] = {row.raw(s)};
+        take<T, ENT, TOP>(a, u, s, step, c);
+    }
+    if (s < row.slots) take_part<T, ENT, TOP>(a, row, s, c);
 }
 
-struct Stat { float r, s, t, mx; };
+struct Stat { float rc, s, t, mx; };
 
-__device__ __forceinline__ Stat join(const Stat& a, const Stat& b, float c) {
+__device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
     Stat o;
-    o.r = fmaxf(a.r, b.r);
-    const float da = a.r == NEG_INF ? -1000.f : floor_y((a.r - o.r) * c), db = b.r == NEG_INF ? -1000.f : floor_y((b.r - o.r) * c);
-    const float fa = ex2(da), fb = ex2(db);
+    o.rc = fmaxf(a.rc, b.rc);
+    const float da = floor_y(a.rc - o.rc), db = floor_y(b.rc - o.rc), fa = ex2(da), fb = ex2(db);
     o.s = fa * a.s + fb * b.s;
-    o.t = fa * (a.t + da * a.s) + fb * (b.t + db * b.s);
+    o.t = fa * fmaf(da, a.s, a.t) + fb * fmaf(db, b.s, b.t);
     o.mx = fmaxf(a.mx, b.mx);
     return o;
 }
 
+struct StatShared { Stat warp[NW], cta[MAX_CLUSTER]; };
+
 // the row's totals, on every thread of the CTA / cluster, joined in the same order everywhere
-__device__ __forceinline__ Stat totals(const Acc& a, float c, Stat* warp_stat, Stat* cta_stat, int cluster, int rank) {
-    Stat st = {a.r, a.s, a.t, a.mx};
+__device__ __forceinline__ Stat totals(const Acc& a, StatShared& sh, int cluster, int rank) {
+    const float s = a.s.x + a.s.y;
+    Stat st = {s == 0.f ? -2.f * FAR : a.rc, s, a.t.x + a.t.y, a.mx};
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) {
         Stat q;
-        q.r = __shfl_xor_sync(~0u, st.r, o); q.s = __shfl_xor_sync(~0u, st.s, o);
+        q.rc = __shfl_xor_sync(~0u, st.rc, o); q.s = __shfl_xor_sync(~0u, st.s, o);
         q.t = __shfl_xor_sync(~0u, st.t, o); q.mx = __shfl_xor_sync(~0u, st.mx, o);
-        st = join(st, q, c);
+        st = join(st, q);
     }
-    if ((threadIdx.x & 31) == 0) warp_stat[threadIdx.x >> 5] = st;
+    if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = st;
     __syncthreads();
-    st = warp_stat[0];
+    st = sh.warp[0];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) st = join(st, warp_stat[w], c);
+    for (int w = 1; w < NW; ++w) st = join(st, sh.warp[w]);
     if (cluster > 1) {
         cg::cluster_group cl = cg::this_cluster();
-        if ((int)threadIdx.x < cluster) cl.map_shared_rank(cta_stat, threadIdx.x)[rank] = st;
+        if ((int)threadIdx.x < cluster) cl.map_shared_rank(&sh, threadIdx.x)->cta[rank] = st;
         cl.sync();
-        st = cta_stat[0];
-        for (int i = 1; i < cluster; ++i) st = join(st, cta_stat[i], c);
+        st = sh.cta[0];
+        for (int i = 1; i < cluster; ++i) st = join(st, sh.cta[i]);
     }
     return st;
 }
 
-// the statistics against the row's maximum: ln S with S >= 1, and sum e (x - m) / S
-struct Final { float m, s, ln_s, mean; };
+// against the row's maximum m: S >= 1, ln S, and mean = sum e (x - m) / S.  A row of -inf is `empty`.
+struct Final { float m, s, ln_s, mean; bool empty; };
+
 __device__ __forceinline__ Final finish(const Stat& st, float c) {
     Final f;
     f.m = st.mx;
-    if (st.mx == NEG_INF && st.s == 0.f) { f.s = 1.f; f.ln_s = 0.f; f.mean = 0.f; return f; }   // only -inf (a NaN makes s NaN)
-    const float dy = (st.r - st.mx) * c, g = ex2(dy);
-    f.s = st.s * g;
+    f.empty = st.mx == NEG_INF && st.s == 0.f;                  // a NaN makes s NaN
+    if (f.empty) { f.s = 1.f; f.ln_s = 0.f; f.mean = 0.f; return f; }
+    const float dy = fmaf(st.mx, c, -st.rc);
+    f.s = st.s * ex2(-dy);
     f.ln_s = logf(f.s);
-    f.mean = LN2 * (st.t / st.s + dy);
+    f.mean = LN2 * (st.t / st.s - dy);
     return f;
+}
+
+// The statistics of a row by the CTA / cluster.  sh[1] serves the second pass of a row beyond NEAR (logits of millions,
+// or nothing but a mask's lowest value), +inf, or -- with an entropy -- f16 whose maximum is so near -65504 (what -inf
+// became) that this would count.
+template <class T, bool ENT, bool TOP>
+__device__ __forceinline__ Final row_statistics(Acc& a, const Row<T>& row, StatShared (&sh)[2], int cluster, int rank, float c) {
+    const int first = rank * TT + threadIdx.x, step = cluster * TT;
+    pass<T, ENT, TOP>(a, row, first, step, c);
+    Stat st = totals(a, sh[0], cluster, rank);
+    const bool low_range = ENT && std::is_same<T, __half>::value && c * (st.mx + 65504.f) < 400.f;
+    if (st.mx != NEG_INF && (fabsf(st.mx) * c >= NEAR || low_range)) {
+        Acc b(c);
+        for (int s = first; s < row.slots; s += step) {
+            float x[Pack<T>::E];
+            if (row.whole(s)) unpack(row.raw(s), x, T()); else row.part(s, x);
+#pragma unroll
+            for (int i = 0; i < Pack<T>::E; ++i) {
+                const float y = (x[i] - st.mx) * c, e = ex2(y);
+                b.s.x += e;
+                if (ENT) b.t.x = fmaf(e, floor_y(y), b.t.x);
+            }
+        }
+        const float m = st.mx;
+        st = totals(b, sh[1], cluster, rank);
+        Final f = {m, st.s, logf(st.s), LN2 * (st.t / st.s), false};
+        return f;
+    }
+    return finish(st, c);
 }
 
 // ---- top alternatives ------------------------------------------------------------------------------
@@ -334,7 +463,7 @@ struct LogprobOut { float *logp, *lse, *entropy, *top; int* top_ids; };
 template <class T, bool TOP>
 __global__ void __launch_bounds__(TT, 4) token_logprob_kernel(const T* __restrict__ z, long long pitch, int v, int k, float scale,
                                                               const void* ids, int wide, LogprobOut out, int cluster) {
-    __shared__ Stat warp_stat[NW], cta_stat[MAX_CLUSTER];
+    __shared__ StatShared stat[2];
     extern __shared__ __align__(16) unsigned char dyn[];
     TopShared& sh = *reinterpret_cast<TopShared*>(dyn);
     const long long n = blockIdx.x / cluster;
@@ -349,19 +478,16 @@ __global__ void __launch_bounds__(TT, 4) token_logprob_kernel(const T* __restric
         there = t >= 0 && t < v;
         if (there) own = to_f(row.p[t]);
     }
-    Acc a;
-    const int first = rank * TT, step = cluster * TT;
-    pass<T, true, TOP>(a, row, first + tid, step, c);
-    const Stat st = totals(a, c, warp_stat, cta_stat, cluster, rank);
-    const Final f = finish(st, c);
-    const bool empty = st.mx == NEG_INF && st.s == 0.f;
+    Acc a(c);
+    const Final f = row_statistics<T, true, TOP>(a, row, stat, cluster, rank, c);
+    const bool empty = f.empty;
     if (rank == 0 && tid == 0) {
         out.logp[n] = !there ? 0.f : empty ? NEG_INF : (own - f.m) * scale - f.ln_s;
         out.lse[n] = f.m * scale + f.ln_s;
         out.entropy[n] = f.ln_s - f.mean;
     }
     if (TOP) {
-        int have = top_of_cta(sh, a, row, first, step, k);
+        int have = top_of_cta(sh, a, row, rank * TT, cluster * TT, k);
         if (cluster > 1) {
             cg::cluster_group cl = cg::this_cluster();
             TopShared* lead = cl.map_shared_rank(&sh, 0);
@@ -556,7 +682,7 @@ template <class T, bool GRAD>
 __global__ void __launch_bounds__(TT, 4) distill_topk_kernel(const T* __restrict__ z, long long pitch, int v, int k, float scale, Teacher te, const float* __restrict__ weights, float* __restrict__ loss,
                                                              T* __restrict__ g, long long g_pitch, int cluster) {
     constexpr int E = Pack<T>::E;
-    __shared__ Stat warp_stat[NW], cta_stat[MAX_CLUSTER];
+    __shared__ StatShared stat[2];
     __shared__ TeacherShared sh;
     const long long n = blockIdx.x / cluster;
     const int rank = blockIdx.x % cluster, tid = threadIdx.x;
@@ -564,11 +690,9 @@ __global__ void __launch_bounds__(TT, 4) distill_topk_kernel(const T* __restrict
     const float c = scale * LOG2E;
     if (cluster > 1) cg::this_cluster().sync();
     if (tid < 32) teacher_row(sh, row.p, v, te, n, k, c);
-    Acc a;
-    pass<T, false, false>(a, row, rank * TT + tid, cluster * TT, c);
-    const Stat st = totals(a, c, warp_stat, cta_stat, cluster, rank);
-    const Final f = finish(st, c);
-    const bool empty = st.mx == NEG_INF && st.s == 0.f;
+    Acc a(c);
+    const Final f = row_statistics<T, false, false>(a, row, stat, cluster, rank, c);
+    const bool empty = f.empty;
     if (rank == 0 && tid < 32) {
         float l = 0.f;
         for (int i = tid; i < k; i += 32) {
