@@ -112,6 +112,7 @@ struct Device {
     int* error_flag_dev = nullptr;
     bool tc_configured = false;
     bool conv_configured = false;
+    unsigned token_configured = 0;   // bit per kernel whose shared-memory limit is raised
 };
 
 // Reference-counted device storage; several buffer handles may share one
@@ -197,10 +198,11 @@ struct TokenShape {
     long long pitch = 0, offset = 0;          // logits, elements
     long long g_pitch = 0, g_offset = 0;      // gradient (or output 0 of a forward kernel: offset only)
     int dtype = EB200_F32, id_dtype = EB200_I32, teacher_dtype = EB200_F32;
-    bool grad = false, entropy = false;
+    bool grad = false, entropy = false, distill = false;
     float scale = 1.f;
     int cluster = 1;                          // CTAs that share a row
     int lanes = 0;                            // > 0: short rows, that many lanes of a warp per row
+    int slice = 0;                            // longer rows: 16-byte slots per CTA
 };
 
 constexpr int KMAX_OUT = 5;

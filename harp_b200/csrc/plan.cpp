@@ -275,6 +275,7 @@ static int plan_token(const eb200_kernel_desc* d, int sm_count, Plan* plan) {
     TokenShape& t = pl.tok;
     t.n = N; t.v = (int)V; t.k = (int)K;
     t.grad = grad;
+    t.distill = distill;
     t.entropy = !distill && (!grad || n_in == 6);
     t.scale = d->scalar;
     // the role of each input: 0 logits, 1 indices, 2 teacher values, 3 a row vector

@@ -13,6 +13,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "tc_ptx.cuh"
 
 namespace eb200 {
 
@@ -25,7 +26,7 @@ constexpr int NW = TT / 32;
 constexpr int MAX_CLUSTER = 8;
 constexpr int MAX_K = 64;                   // alternatives
 constexpr int GROUPS = 64;                  // groups of threads whose maxima bound the k-th largest logit, >= MAX_K
-constexpr int CAP = 1024;                   // candidates held at a time
+constexpr int CAP = 512;                    // candidates held at a time, >= MAX_CLUSTER * MAX_K
 constexpr int MAX_TEACHER = 256;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
@@ -222,12 +223,11 @@ __device__ __forceinline__ void take(Acc& a, const uint4 (&u)[N], int slot, int 
 
 // a slot that reaches over the row's ends (its places outside hold -inf)
 template <class T, bool ENT, bool TOP>
-__device__ __forceinline__ void take_part(Acc& a, const Row<T>& row, int slot, float c) {
-    float x[Pack<T>::E], mx = NEG_INF;
-    row.part(slot, x);
+__device__ __forceinline__ void take_part(Acc& a, const float (&x)[Pack<T>::E], int slot, float c) {
+    float mx = NEG_INF;
 #pragma unroll
     for (int i = 0; i < Pack<T>::E; ++i) mx = fmaxf(mx, x[i]);
-    if (TOP && mx > a.mx) a.slot = slot;
+    if (TOP && (mx > a.mx || (mx == a.mx && slot < a.slot))) a.slot = slot;      // the row's first slot is taken last
     a.mx = fmaxf(a.mx, mx);
     if (mx > a.lim) move_reference(a, mx, c);
 #pragma unroll
@@ -236,27 +236,6 @@ __device__ __forceinline__ void take_part(Acc& a, const Row<T>& row, int slot, f
         a.s.x += e;
         if (ENT) a.t.x = fmaf(e, floor_y(y), a.t.x);
     }
-}
-
-// this thread's share of a row: slots first, first + step, ...
-template <class T, bool ENT, bool TOP>
-__device__ __forceinline__ void pass(Acc& a, const Row<T>& row, int first, int step, float c) {
-    constexpr int U = 4;
-    int s = first;
-    if (s < row.slots) a.slot = s;
-    if (s < row.slots && !row.whole(s)) { take_part<T, ENT, TOP>(a, row, s, c); s += step; }
-    const int end = row.whole(row.slots - 1) ? row.slots : row.slots - 1;
-    for (; s + (U - 1) * step < end; s += U * step) {
-        uint4 u[U];
-#pragma unroll
-        for (int i = 0; i < U; ++i) u[i] = row.raw(s + i * step);
-        take<T, ENT, TOP>(a, u, s, step, c);
-    }
-    for (; s < end; s += step) {
-        const uint4 u[1] = {row.raw(s)};
-        take<T, ENT, TOP>(a, u, s, step, c);
-    }
-    if (s < row.slots) take_part<T, ENT, TOP>(a, row, s, c);
 }
 
 struct Stat { float rc, s, t, mx; };
@@ -271,10 +250,14 @@ __device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
     return o;
 }
 
-struct StatShared { Stat warp[NW], cta[MAX_CLUSTER]; };
+template <int CT> struct StatShared { Stat warp[CT / 32], cta[MAX_CLUSTER]; };
 
-// the row's totals, on every thread of the CTA / cluster, joined in the same order everywhere
-__device__ __forceinline__ Stat totals(const Acc& a, StatShared& sh, int cluster, int rank) {
+// the barrier of the CT threads that take logits
+template <int CT> __device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, %0;" ::"n"(CT) : "memory"); }
+
+// the CTA's totals on all those threads, joined in the same order everywhere
+template <int CT>
+__device__ __forceinline__ Stat cta_totals(const Acc& a, StatShared<CT>& sh) {
     const float s = a.s.x + a.s.y;
     Stat st = {s == 0.f ? -2.f * FAR : a.rc, s, a.t.x + a.t.y, a.mx};
 #pragma unroll
@@ -285,17 +268,42 @@ __device__ __forceinline__ Stat totals(const Acc& a, StatShared& sh, int cluster
         st = join(st, q);
     }
     if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = st;
-    __syncthreads();
+    rows_sync<CT>();
     st = sh.warp[0];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) st = join(st, sh.warp[w]);
-    if (cluster > 1) {
-        cg::cluster_group cl = cg::this_cluster();
-        if ((int)threadIdx.x < cluster) cl.map_shared_rank(&sh, threadIdx.x)->cta[rank] = st;
-        cl.sync();
-        st = sh.cta[0];
-        for (int i = 1; i < cluster; ++i) st = join(st, sh.cta[i]);
+    for (int w = 1; w < CT / 32; ++w) st = join(st, sh.warp[w]);
+    return st;
+}
+
+// The CTAs of a cluster hand each other their totals (and CTA 0 their alternatives): plain stores into the peer's
+// shared memory, then an arrival at the peer's mbarrier.  Every CTA waits for all the others' before it ends, so no
+// store reaches a CTA that has gone.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ void arrive_at(uint64_t* bar, int cta) {
+    asm volatile("{ .reg .b32 a; mapa.shared::cluster.u32 a, %0, %1; mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a]; }"
+                 ::"r"(smem_u32(bar)), "r"(cta) : "memory");
+}
+__device__ __forceinline__ void wait_cluster(uint64_t* bar, int* error_flag) {
+    for (unsigned i = 0; i < TC_SPIN_LIMIT; ++i) {
+        unsigned ok;
+        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0; selp.u32 %0, 1, 0, p; }"
+                     : "=r"(ok) : "r"(smem_u32(bar)) : "memory");
+        if (ok) return;
+        if (i > 4096) __nanosleep(64);
     }
+    atomicExch(error_flag, 1);
+}
+
+template <int CT>
+__device__ __forceinline__ Stat exchange(const Stat& mine, StatShared<CT>& sh, uint64_t* bar, int cluster, int rank, int* error_flag) {
+    const int tid = threadIdx.x;
+    if (tid < cluster) cg::this_cluster().map_shared_rank(&sh, tid)->cta[rank] = mine;
+    rows_sync<CT>();                        // all stores of this CTA lie before its arrivals
+    if (tid < cluster) arrive_at(bar, tid);
+    wait_cluster(bar, error_flag);
+    Stat st = sh.cta[0];
+    for (int i = 1; i < cluster; ++i) st = join(st, sh.cta[i]);
     return st;
 }
 
@@ -314,34 +322,22 @@ __device__ __forceinline__ Final finish(const Stat& st, float c) {
     return f;
 }
 
-// The statistics of a row by the CTA / cluster.  sh[1] serves the second pass of a row beyond NEAR (logits of millions,
-// or nothing but a mask's lowest value), +inf, or -- with an entropy -- f16 whose maximum is so near -65504 (what -inf
-// became) that this would count.
-template <class T, bool ENT, bool TOP>
-__device__ __forceinline__ Final row_statistics(Acc& a, const Row<T>& row, StatShared (&sh)[2], int cluster, int rank, float c) {
-    const int first = rank * TT + threadIdx.x, step = cluster * TT;
-    pass<T, ENT, TOP>(a, row, first, step, c);
-    Stat st = totals(a, sh[0], cluster, rank);
-    const bool low_range = ENT && std::is_same<T, __half>::value && c * (st.mx + 65504.f) < 400.f;
-    if (st.mx != NEG_INF && (fabsf(st.mx) * c >= NEAR || low_range)) {
-        Acc b(c);
-        for (int s = first; s < row.slots; s += step) {
-            float x[Pack<T>::E];
-            if (row.whole(s)) unpack(row.raw(s), x, T()); else row.part(s, x);
-#pragma unroll
-            for (int i = 0; i < Pack<T>::E; ++i) {
-                const float y = (x[i] - st.mx) * c, e = ex2(y);
-                b.s.x += e;
-                if (ENT) b.t.x = fmaf(e, floor_y(y), b.t.x);
-            }
-        }
-        const float m = st.mx;
-        st = totals(b, sh[1], cluster, rank);
-        Final f = {m, st.s, logf(st.s), LN2 * (st.t / st.s), false};
-        return f;
-    }
-    return finish(st, c);
+// Rows that are summed again against their maximum: beyond NEAR (logits of millions, or nothing but a mask's lowest
+// value), +inf, or -- with an entropy -- f16 whose maximum is so near -65504 (what -inf became) that this would count.
+template <class T, bool ENT> __device__ __forceinline__ bool again(float m, float c) {
+    const bool low_range = ENT && std::is_same<T, __half>::value && c * (m + 65504.f) < 400.f;
+    return m != NEG_INF && (fabsf(m) * c >= NEAR || low_range);
 }
+
+template <bool ENT, int E> __device__ __forceinline__ void take_against(Acc& b, const float (&x)[E], float m, float c) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const float y = (x[i] - m) * c, e = ex2(y);
+        b.s.x += e;
+        if (ENT) b.t.x = fmaf(e, floor_y(y), b.t.x);
+    }
+}
+__device__ __forceinline__ Final finish_against(const Stat& st, float m) { return {m, st.s, logf(st.s), LN2 * (st.t / st.s), false}; }
 
 // ---- top alternatives ------------------------------------------------------------------------------
 // Order of a logit as an unsigned whole number (NaN like -inf, -0 like 0); 0 is below every logit.
@@ -367,7 +363,7 @@ __device__ __forceinline__ int keep_largest(TopShared& sh, int n, int k) {
     constexpr int PER = CAP / TT;
     unsigned long long mine[PER];
     int rank[PER];
-    __syncthreads();
+    rows_sync<TT>();
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int at = threadIdx.x + i * TT;
@@ -379,32 +375,33 @@ __device__ __forceinline__ int keep_largest(TopShared& sh, int n, int k) {
             rank[i] = r;
         }
     }
-    __syncthreads();
+    rows_sync<TT>();
 #pragma unroll
     for (int i = 0; i < PER; ++i)
         if (rank[i] < k) sh.cand[rank[i]] = mine[i];
-    __syncthreads();
+    rows_sync<TT>();
     return min(n, k);
 }
 
 // The k largest logits of this CTA's slots (first + tid + i * step) into sh.cand, sorted; returns how many.
 // The k-th largest of 64 group maxima bounds the k-th largest logit from below, so only threads whose
 // maximum reaches it hold candidates; their slots (about 1.3 k threads' worth) are read again, by all threads.
-template <class T>
-__device__ __forceinline__ int top_of_cta(TopShared& sh, const Acc& a, const Row<T>& row, int first, int step, int k) {
+// get(s, x) brings slot s < end.
+template <class T, class GET>
+__device__ __forceinline__ int top_of_cta(TopShared& sh, const Acc& a, const Row<T>& row, int first, int step, int end, int k, GET get) {
     constexpr int E = Pack<T>::E;
     const int tid = threadIdx.x;
     const unsigned long long key = a.slot < 0 ? 0 : key_of(order_of(a.mx), a.slot);
     sh.keys[tid] = key;
     if (tid == 0) sh.n_owners = sh.n_cand = 0;
-    __syncthreads();
+    rows_sync<TT>();
     if (tid < GROUPS) {
         unsigned long long g = 0;
 #pragma unroll
         for (int i = 0; i < TT / GROUPS; ++i) g = max(g, sh.keys[tid + i * GROUPS]);
         sh.groups[tid] = g;
     }
-    __syncthreads();
+    rows_sync<TT>();
     if (tid < GROUPS) {
         const unsigned long long g = sh.groups[tid];
         int r = 0;
@@ -412,19 +409,19 @@ __device__ __forceinline__ int top_of_cta(TopShared& sh, const Acc& a, const Row
         for (int j = 0; j < GROUPS; ++j) r += sh.groups[j] > g || (sh.groups[j] == g && j < tid);
         if (r == k - 1) sh.tau = g;
     }
-    __syncthreads();
+    rows_sync<TT>();
     const unsigned long long tau = sh.tau;
     const unsigned tau_order = (unsigned)(tau >> 32);
     const int tau_slot = (int)(0xffffffffu - (unsigned)tau);       // equal values count up to the end of this slot
     if (key != 0 && key >= tau) sh.owners[atomicAdd(&sh.n_owners, 1)] = tid;
-    __syncthreads();
-    const int n_own = sh.n_owners, per = (row.slots - first + step - 1) / step;
+    rows_sync<TT>();
+    const int n_own = sh.n_owners, per = (end - first + step - 1) / step;
     const long long pairs = (long long)n_own * per;
     auto collect = [&](long long pair) {
         const int s = first + sh.owners[(int)(pair % n_own)] + (int)(pair / n_own) * step;
-        if (s >= row.slots) return;
+        if (s >= end) return;
         float x[E];
-        if (row.whole(s)) unpack(row.raw(s), x, T()); else row.part(s, x);
+        get(s, x);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             const unsigned o = order_of(x[i]);
@@ -436,19 +433,19 @@ __device__ __forceinline__ int top_of_cta(TopShared& sh, const Acc& a, const Row
         }
     };
     for (long long p = tid; p < pairs; p += TT) collect(p);
-    __syncthreads();
+    rows_sync<TT>();
     int n = sh.n_cand;
     if (n > CAP) {
         // more than fit (large logits gathered in a few threads' slots): some slots at a time, keeping the k largest
         constexpr int CHUNK = (CAP - MAX_K) / E / 32 * 32;
         n = 0;
         for (long long p0 = 0; p0 < pairs; p0 += CHUNK) {
-            __syncthreads();
+            rows_sync<TT>();
             if (tid == 0) sh.n_cand = n;
-            __syncthreads();
+            rows_sync<TT>();
             const long long p1 = min(p0 + CHUNK, pairs);
             for (long long p = p0 + tid; p < p1; p += TT) collect(p);
-            __syncthreads();
+            rows_sync<TT>();
             n = keep_largest(sh, sh.n_cand, k);
         }
         return n;
@@ -456,60 +453,24 @@ __device__ __forceinline__ int top_of_cta(TopShared& sh, const Acc& a, const Row
     return keep_largest(sh, n, k);
 }
 
+// The CTAs' candidates at CTA 0 of the cluster: sent, and after a cluster barrier merged there.
+__device__ __forceinline__ void send_top(TopShared& sh, int have, int rank) {
+    TopShared* lead = cg::this_cluster().map_shared_rank(&sh, 0);
+    if ((int)threadIdx.x < have) lead->peers[rank * MAX_K + threadIdx.x] = sh.cand[threadIdx.x];
+    if (threadIdx.x == 0) lead->n_peers[rank] = have;
+}
+__device__ __forceinline__ void merge_top(TopShared& sh, int cluster, int k) {
+    if (threadIdx.x == 0) sh.n_cand = 0;
+    rows_sync<TT>();
+    for (int i = threadIdx.x; i < cluster * MAX_K; i += TT)
+        if (i % MAX_K < sh.n_peers[i / MAX_K]) sh.cand[atomicAdd(&sh.n_cand, 1)] = sh.peers[i];
+    rows_sync<TT>();
+    keep_largest(sh, sh.n_cand, k);
+}
+
 // ---- forward ---------------------------------------------------------------------------------------
 
 struct LogprobOut { float *logp, *lse, *entropy, *top; int* top_ids; };
-
-template <class T, bool TOP>
-__global__ void __launch_bounds__(TT, 4) token_logprob_kernel(const T* __restrict__ z, long long pitch, int v, int k, float scale,
-                                                              const void* ids, int wide, LogprobOut out, int cluster) {
-    __shared__ StatShared stat[2];
-    extern __shared__ __align__(16) unsigned char dyn[];
-    TopShared& sh = *reinterpret_cast<TopShared*>(dyn);
-    const long long n = blockIdx.x / cluster;
-    const int rank = blockIdx.x % cluster, tid = threadIdx.x;
-    const Row<T> row(z + n * pitch, v);
-    const float c = scale * LOG2E;
-    if (cluster > 1) cg::this_cluster().sync();       // every CTA of the cluster runs before its memory is written
-    float own = NEG_INF;
-    bool there = false;
-    if (rank == 0 && tid == 0) {
-        const long long t = load_id(ids, n, wide);
-        there = t >= 0 && t < v;
-        if (there) own = to_f(row.p[t]);
-    }
-    Acc a(c);
-    const Final f = row_statistics<T, true, TOP>(a, row, stat, cluster, rank, c);
-    const bool empty = f.empty;
-    if (rank == 0 && tid == 0) {
-        out.logp[n] = !there ? 0.f : empty ? NEG_INF : (own - f.m) * scale - f.ln_s;
-        out.lse[n] = f.m * scale + f.ln_s;
-        out.entropy[n] = f.ln_s - f.mean;
-    }
-    if (TOP) {
-        int have = top_of_cta(sh, a, row, rank * TT, cluster * TT, k);
-        if (cluster > 1) {
-            cg::cluster_group cl = cg::this_cluster();
-            TopShared* lead = cl.map_shared_rank(&sh, 0);
-            if (tid < have) lead->peers[rank * MAX_K + tid] = sh.cand[tid];
-            if (tid == 0) lead->n_peers[rank] = have;
-            cl.sync();
-            if (rank != 0) return;
-            __syncthreads();
-            if (tid == 0) sh.n_cand = 0;
-            __syncthreads();
-            for (int i = tid; i < cluster * MAX_K; i += TT)
-                if (i % MAX_K < sh.n_peers[i / MAX_K]) sh.cand[atomicAdd(&sh.n_cand, 1)] = sh.peers[i];
-            __syncthreads();
-            have = keep_largest(sh, sh.n_cand, k);
-        }
-        if (tid < k) {
-            const unsigned long long key = sh.cand[tid];
-            out.top[n * k + tid] = empty ? NEG_INF : (value_of((unsigned)(key >> 32)) - f.m) * scale - f.ln_s;
-            out.top_ids[n * k + tid] = (int)index_of(key);
-        }
-    }
-}
 
 // ---- 16 bytes of logits from any element address ---------------------------------------------------
 
@@ -570,23 +531,34 @@ template <class T> __device__ __forceinline__ void put(T* p, int v, int j, const
 // A warp takes 32 * GU slots of a row.
 constexpr int GU = 4;
 
+struct GradArgs {
+    const void* z;
+    void* g;
+    long long pitch, g_pitch, rows;
+    int v, per_row;
+    float scale;
+    const void* ids;
+    int wide;
+    const float *lse, *g_logp, *entropy, *g_entropy;
+};
+
 template <class T, bool ENT>
-__global__ void __launch_bounds__(TT) token_logprob_grad_kernel(const T* __restrict__ z, long long pitch, T* __restrict__ g, long long g_pitch, long long rows, int v,
-                                                                float scale, const void* ids, int wide, const float* __restrict__ lse, const float* __restrict__ g_logp,
-                                                                const float* __restrict__ entropy, const float* __restrict__ g_entropy, int per_row) {
+__global__ void __launch_bounds__(TT) token_logprob_grad_kernel(const GradArgs a) {
     constexpr int E = Pack<T>::E;
+    const int per_row = a.per_row, v = a.v;
+    const float scale = a.scale;
     const long long task = (long long)blockIdx.x * NW + (threadIdx.x >> 5);
     const long long n = task / per_row;
-    if (n >= rows) return;
+    if (n >= a.rows) return;
     const int lane = threadIdx.x & 31, s0 = (int)(task % per_row) * 32 * GU + lane;
-    const T* p = z + n * pitch;
-    T* o = g + n * g_pitch;
+    const T* p = reinterpret_cast<const T*>(a.z) + n * a.pitch;
+    T* o = reinterpret_cast<T*>(a.g) + n * a.g_pitch;
     const int lead = (int)((reinterpret_cast<uintptr_t>(o) & 15) / sizeof(T));
     const int slots = (lead + v + E - 1) / E;
     const int shift = (int)(reinterpret_cast<uintptr_t>(p - lead) & 15);
-    const long long t = load_id(ids, n, wide);
-    const float norm = __ldg(lse + n), gl = t >= 0 && t < v ? __ldg(g_logp + n) : 0.f;
-    const float gh = ENT ? __ldg(g_entropy + n) : 0.f, h = ENT ? __ldg(entropy + n) : 0.f;
+    const long long t = load_id(a.ids, n, a.wide);
+    const float norm = __ldg(a.lse + n), gl = t >= 0 && t < v ? __ldg(a.g_logp + n) : 0.f;
+    const float gh = ENT ? __ldg(a.g_entropy + n) : 0.f, h = ENT ? __ldg(a.entropy + n) : 0.f;
     const bool zero = norm == NEG_INF || (gl == 0.f && gh == 0.f);
     const float up = gl * scale, al = -up, ah = -gh * scale;
     Window<T> w[GU];
@@ -678,63 +650,298 @@ __device__ __forceinline__ void teacher_row(TeacherShared& sh, const T* p, int v
     if (lane == 0) sh.some = s != 0.f;        // NaN counts
 }
 
-template <class T, bool GRAD>
-__global__ void __launch_bounds__(TT, 4) distill_topk_kernel(const T* __restrict__ z, long long pitch, int v, int k, float scale, Teacher te, const float* __restrict__ weights, float* __restrict__ loss,
-                                                             T* __restrict__ g, long long g_pitch, int cluster) {
-    constexpr int E = Pack<T>::E;
-    __shared__ StatShared stat[2];
-    __shared__ TeacherShared sh;
-    const long long n = blockIdx.x / cluster;
-    const int rank = blockIdx.x % cluster, tid = threadIdx.x;
-    const Row<T> row(z + n * pitch, v);
-    const float c = scale * LOG2E;
-    if (cluster > 1) cg::this_cluster().sync();
-    if (tid < 32) teacher_row(sh, row.p, v, te, n, k, c);
-    Acc a(c);
-    const Final f = row_statistics<T, false, false>(a, row, stat, cluster, rank, c);
-    const bool empty = f.empty;
-    if (rank == 0 && tid < 32) {
-        float l = 0.f;
-        for (int i = tid; i < k; i += 32) {
-            const float q = sh.q[i], lp = empty ? NEG_INF : (sh.z[i] - f.m) * scale - f.ln_s;
-            if (!(q == 0.f)) l += q * (sh.ln_q[i] - lp);
-        }
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
-        if (tid == 0) loss[n] = l;
+// by one warp
+__device__ __forceinline__ float distill_loss(const TeacherShared& sh, const Final& f, int k, float scale) {
+    float l = 0.f;
+    for (int i = threadIdx.x & 31; i < k; i += 32) {
+        const float q = sh.q[i], lp = f.empty ? NEG_INF : (sh.z[i] - f.m) * scale - f.ln_s;
+        if (!(q == 0.f)) l += q * (sh.ln_q[i] - lp);
     }
-    if (!GRAD) return;
-    const float w = __ldg(weights + n);
-    const bool zero = w == 0.f || empty || !sh.some;
-    const float up = w * scale, fac = up / f.s;
-    T* o = g + n * g_pitch;
-    const int lead = (int)((reinterpret_cast<uintptr_t>(o) & 15) / sizeof(T));
-    const int slots = (lead + v + E - 1) / E;
-    const int shift = (int)(reinterpret_cast<uintptr_t>(row.p - lead) & 15);
-    for (int s = rank * TT + tid; s < slots; s += cluster * TT) {
-        const int j = s * E - lead;
-        float x[E];
-        if (zero) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = 0.f;
-        } else {
-            Window<T> win;
-            win.load(row.p, v, j, shift);
-            win.get(x, shift);
-#pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = ex2((x[i] - f.m) * c) * fac;
-        }
-        put(o, v, j, x);
+    for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+    return l;
+}
+
+// ---- longer rows -----------------------------------------------------------------------------------
+// CTAs that stay take rows in turn.  One thread keeps a ring of chunks in shared memory filled by bulk copies, running
+// ahead into the next row while this one is being finished, so what is in flight depends neither on registers nor on
+// where a row ends; one warp fetches what else a row needs (the token's logit, the teacher's entries), a row ahead;
+// CT threads take the logits.  Few rows: the CTAs of a cluster share one, each a slice of whole slots.
+// The distillation gradient has the row's chunks brought a second time, which L2 serves: the rows in work at a time are
+// a fraction of it.
+enum { ROWS_LOGPROB, ROWS_TOP, ROWS_DISTILL, ROWS_DISTILL_GRAD };
+
+struct RowsArgs {
+    const void* z;
+    long long pitch, rows;
+    int v, k;
+    float scale;
+    const void* ids;
+    int wide;
+    LogprobOut out;
+    Teacher te;
+    const float* weights;
+    float* loss;
+    void* g;
+    long long g_pitch;
+    int cluster, per;                       // slots per CTA of a row
+    int* error_flag;
+};
+
+template <int MODE> struct RowsShape {
+    static constexpr int CT = MODE == ROWS_DISTILL_GRAD ? 512 : TT;       // threads that take logits
+    static constexpr int CTAS = MODE == ROWS_DISTILL_GRAD ? 1 : 3;        // per SM
+    static constexpr int CHUNK = 4 * CT;                                  // slots per copy: 16 or 32 KB
+    static constexpr int STAGES = MODE == ROWS_DISTILL_GRAD ? 6 : MODE == ROWS_TOP ? 3 : 4;
+    static constexpr int STAGE_BYTES = CHUNK * 16 + (MODE == ROWS_DISTILL_GRAD ? 128 : 0);      // one more slot for windows over the chunk's end
+    static constexpr int THREADS = CT + 64;                               // and the copying thread's warp, and the fetching one
+};
+
+struct OwnLogit { float z; int there; };
+struct Edges { uint4 head, tail; };          // the row's slots that reach over its ends
+
+template <int MODE> struct RowsShared {
+    using S = RowsShape<MODE>;
+    unsigned char ring[S::STAGES][S::STAGE_BYTES];
+    uint64_t full[S::STAGES], empty[S::STAGES], side_full[2], side_empty[2], peers[2];
+    alignas(16) StatShared<S::CT> stat[2], second;
+    Edges edges[2];
+    OwnLogit own[2];
+    float weight[2];
+    TeacherShared teach[MODE >= ROWS_DISTILL ? 2 : 1];
+};
+template <> struct RowsShared<ROWS_TOP> {
+    using S = RowsShape<ROWS_TOP>;
+    unsigned char ring[S::STAGES][S::STAGE_BYTES];
+    uint64_t full[S::STAGES], empty[S::STAGES], side_full[2], side_empty[2], peers[2];
+    alignas(16) StatShared<S::CT> stat[2], second;
+    Edges edges[2];
+    OwnLogit own[2];
+    TopShared top;
+};
+
+// the whole slots [w0, w1) among the m slots of this CTA's slice, which begins at slot `first`
+struct Slice {
+    int first, m, w0, w1;
+    __device__ bool tail() const { return w1 < m && m - 1 >= w0; }
+};
+template <class T> __device__ __forceinline__ Slice slice_of(const Row<T>& row, int rank, int per) {
+    Slice s;
+    s.first = rank * per;
+    s.m = max(0, min(row.slots - s.first, per));
+    s.w0 = s.m > 0 && !row.whole(s.first) ? 1 : 0;
+    s.w1 = s.m > 0 && !row.whole(s.first + s.m - 1) ? max(s.m - 1, s.w0) : s.m;
+    return s;
+}
+
+template <class T, int MODE>
+__global__ void __launch_bounds__(RowsShape<MODE>::THREADS, RowsShape<MODE>::CTAS) token_rows_kernel(const RowsArgs a) {
+    using S = RowsShape<MODE>;
+    constexpr int E = Pack<T>::E, CT = S::CT, CHUNK = S::CHUNK, STAGES = S::STAGES, U = CHUNK / CT;
+    constexpr bool TOP = MODE == ROWS_TOP, ENT = MODE <= ROWS_TOP, DISTILL = MODE >= ROWS_DISTILL, GRAD = MODE == ROWS_DISTILL_GRAD;
+    extern __shared__ __align__(128) unsigned char dyn[];
+    RowsShared<MODE>& sh = *reinterpret_cast<RowsShared<MODE>*>(dyn);
+    const int tid = threadIdx.x, warp = tid >> 5, cluster = a.cluster, rank = blockIdx.x % cluster;
+    const long long n0 = blockIdx.x / cluster, step = gridDim.x / cluster;
+    const float c = a.scale * LOG2E;
+
+    if (tid == 0) {
+        for (int i = 0; i < STAGES; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], CT / 32); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sh.side_full[i], 1); mbar_init(&sh.side_empty[i], CT / 32); mbar_init(&sh.peers[i], cluster); }
+        asm volatile("fence.mbarrier_init.release.cluster; fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (zero) return;
     __syncthreads();
-    if (tid < k) {
-        const int id = sh.id[tid];
-        if (id >= 0 && ((id + lead) / E / TT) % cluster == rank) {
-            float q = 0.f;
-            for (int i = 0; i < k; ++i) q += sh.id[i] == id ? sh.q[i] : 0.f;
-            o[id] = from_f<T>(ex2((sh.z[tid] - f.m) * c) * fac - up * q);
+    if (cluster > 1) cluster_arrive();      // waited for before the first store into another CTA
+
+    if (warp == CT / 32) {                  // ---- copies ----
+        if ((tid & 31) == 0) {
+            unsigned it = 0;
+            for (long long n = n0; n < a.rows; n += step) {
+                const Row<T> row(reinterpret_cast<const T*>(a.z) + n * a.pitch, a.v);
+                const Slice sl = slice_of(row, rank, a.per);
+                const uint4* src = reinterpret_cast<const uint4*>(row.p - row.lead) + sl.first;
+                for (int round = 0; round < (GRAD ? 2 : 1); ++round) {
+                    for (int lo = 0; lo < sl.w1; lo += CHUNK, ++it) {
+                        const int st = it % STAGES, b = max(lo, sl.w0), e = min(lo + CHUNK + (round ? 1 : 0), sl.w1);
+                        if (it >= STAGES) mbar_wait(&sh.empty[st], (it / STAGES - 1) & 1, a.error_flag);
+                        const unsigned bytes = e > b ? (e - b) * 16 : 0;
+                        mbar_expect_tx(&sh.full[st], bytes);
+                        if (bytes) bulk_load(sh.ring[st] + (b - lo) * 16, src + b, bytes, &sh.full[st]);
+                    }
+                }
+            }
         }
+        __syncwarp();
+        if (cluster > 1) cluster_wait();
+        return;
+    }
+    if (warp == CT / 32 + 1) {              // ---- what else a row needs ----
+        const int lane = tid & 31;
+        unsigned it = 0;
+        for (long long n = n0; n < a.rows; n += step, ++it) {
+            const int b = it & 1;
+            const T* p = reinterpret_cast<const T*>(a.z) + n * a.pitch;
+            const Row<T> row(p, a.v);
+            const Slice sl = slice_of(row, rank, a.per);
+            if (it >= 2) mbar_wait(&sh.side_empty[b], (it / 2 - 1) & 1, a.error_flag);
+            if ((lane == 1 && sl.w0 == 1) || (lane == 2 && sl.tail())) {
+                float x[E];
+                row.part(lane == 1 ? sl.first : sl.first + sl.m - 1, x);
+                (lane == 1 ? sh.edges[b].head : sh.edges[b].tail) = pack(x, T());
+            }
+            if constexpr (DISTILL) {
+                teacher_row(sh.teach[b], p, a.v, a.te, n, a.k, c);
+                if (GRAD && lane == 0) sh.weight[b] = __ldg(a.weights + n);
+            } else if (lane == 0) {
+                const long long t = load_id(a.ids, n, a.wide);
+                const bool there = t >= 0 && t < a.v;
+                sh.own[b] = {there ? to_f(__ldg(p + t)) : NEG_INF, there};
+            }
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&sh.side_full[b])) : "memory");
+        }
+        if (cluster > 1) cluster_wait();
+        return;
+    }
+
+    // ---- logits ----
+    auto arrive = [&](uint64_t* bar) {      // by a warp
+        __syncwarp();
+        if ((tid & 31) == 0) asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+    };
+    unsigned it = 0, turn = 0;
+    for (long long n = n0; n < a.rows; n += step, ++turn) {
+        const Row<T> row(reinterpret_cast<const T*>(a.z) + n * a.pitch, a.v);
+        const Slice sl = slice_of(row, rank, a.per);
+        const int b = turn & 1;
+        Acc acc(c);
+        acc.slot = tid < sl.m ? sl.first + tid : -1;
+        for (int lo = 0; lo < sl.w1; lo += CHUNK, ++it) {
+            const int st = it % STAGES;
+            const uint4* chunk = reinterpret_cast<const uint4*>(sh.ring[st]);
+            mbar_wait(&sh.full[st], (it / STAGES) & 1, a.error_flag);
+            if (lo >= sl.w0 && lo + CHUNK <= sl.w1) {
+                uint4 u[U];
+#pragma unroll
+                for (int q = 0; q < U; ++q) u[q] = chunk[tid + q * CT];
+                arrive(&sh.empty[st]);
+                take<T, ENT, TOP>(acc, u, sl.first + lo + tid, CT, c);
+            } else {
+                for (int s = tid; s < CHUNK; s += CT) {
+                    if (lo + s < sl.w0 || lo + s >= sl.w1) continue;
+                    const uint4 u[1] = {chunk[s]};
+                    take<T, ENT, TOP>(acc, u, sl.first + lo + s, CT, c);
+                }
+                arrive(&sh.empty[st]);
+            }
+        }
+        mbar_wait(&sh.side_full[b], (turn / 2) & 1, a.error_flag);
+        // the slots over the row's ends, by the threads whose turn their places are
+        if (sl.w0 == 1 && tid == 0) { float x[E]; unpack(sh.edges[b].head, x, T()); take_part<T, ENT, TOP>(acc, x, sl.first, c); }
+        if (sl.tail() && tid == (sl.m - 1) % CT) { float x[E]; unpack(sh.edges[b].tail, x, T()); take_part<T, ENT, TOP>(acc, x, sl.first + sl.m - 1, c); }
+        __syncwarp();
+
+        Stat st = cta_totals<CT>(acc, sh.stat[b]);
+        if constexpr (TOP) {
+            const int have = top_of_cta(sh.top, acc, row, sl.first, TT, sl.first + sl.m, a.k,
+                                        [&](int s, float (&x)[E]) { if (row.whole(s)) unpack(row.raw(s), x, T()); else row.part(s, x); });
+            if (cluster > 1) { cluster_wait(); send_top(sh.top, have, rank); }
+        } else {
+            if (cluster > 1) cluster_wait();
+        }
+        if (cluster > 1) st = exchange<CT>(st, sh.stat[b], &sh.peers[0], cluster, rank, a.error_flag);
+        Final f;
+        if (again<T, ENT>(st.mx, c)) {
+            Acc sec(c);
+            for (int s = sl.first + tid; s < sl.first + sl.m; s += CT) {
+                float x[E];
+                if (row.whole(s)) unpack(row.raw(s), x, T()); else row.part(s, x);
+                take_against<ENT>(sec, x, st.mx, c);
+            }
+            rows_sync<CT>();                // sh.second may still be read for the row before
+            Stat st2 = cta_totals<CT>(sec, sh.second);
+            if (cluster > 1) st2 = exchange<CT>(st2, sh.second, &sh.peers[1], cluster, rank, a.error_flag);
+            f = finish_against(st2, st.mx);
+        } else {
+            f = finish(st, c);
+        }
+
+        if constexpr (!DISTILL) {
+            if (rank == 0 && tid == 0) {
+                const OwnLogit own = sh.own[b];
+                a.out.logp[n] = !own.there ? 0.f : f.empty ? NEG_INF : (own.z - f.m) * a.scale - f.ln_s;
+                a.out.lse[n] = f.m * a.scale + f.ln_s;
+                a.out.entropy[n] = f.ln_s - f.mean;
+            }
+            if constexpr (TOP) {
+                if (rank == 0) {
+                    if (cluster > 1) merge_top(sh.top, cluster, a.k);
+                    if (tid < a.k) {
+                        const unsigned long long key = sh.top.cand[tid];
+                        a.out.top[n * a.k + tid] = f.empty ? NEG_INF : (value_of((unsigned)(key >> 32)) - f.m) * a.scale - f.ln_s;
+                        a.out.top_ids[n * a.k + tid] = (int)index_of(key);
+                    }
+                }
+            }
+        } else {
+            const TeacherShared& teach = sh.teach[b];
+            if (rank == 0 && warp == 0) {
+                const float l = distill_loss(teach, f, a.k, a.scale);
+                if (tid == 0) a.loss[n] = l;
+            }
+            if constexpr (GRAD) {
+                const float w = sh.weight[b];
+                const bool zero = w == 0.f || f.empty || !teach.some;
+                const float up = w * a.scale, fac = up / f.s;
+                // logit j at element j - base of the slice; stores along the output's own slots
+                T* o = reinterpret_cast<T*>(a.g) + n * a.g_pitch;
+                const int lead = (int)((reinterpret_cast<uintptr_t>(o) & 15) / sizeof(T));
+                const int base = sl.first * E - row.lead, end = base + sl.w1 * E;       // [.., end): the whole slots' logits
+                auto slot_at = [&](int j) { return (j + lead + E - 1) / E; };           // first output slot that begins at j or later
+                for (int lo = 0; lo < sl.w1; lo += CHUNK, ++it) {
+                    const int st = it % STAGES;
+                    const uint4* chunk = reinterpret_cast<const uint4*>(sh.ring[st]);
+                    const int from = max(lo, sl.w0), to = min(lo + CHUNK, sl.w1);
+                    const int s0 = slot_at(base + from * E), s1 = to == sl.w1 ? (end + lead) / E : slot_at(base + to * E);
+                    const int off = s0 * E - lead - (base + lo * E), shift = off % E * (int)sizeof(T);
+                    const uint4* win = chunk + off / E;
+                    uint4* dst = reinterpret_cast<uint4*>(o - lead) + s0;
+                    mbar_wait(&sh.full[st], (it / STAGES) & 1, a.error_flag);
+                    for (int i = tid; i < s1 - s0; i += CT) {
+                        float x[E];
+                        if (zero) {
+#pragma unroll
+                            for (int q = 0; q < E; ++q) x[q] = 0.f;
+                        } else {
+                            if (shift == 0) unpack(win[i], x, T()); else unpack(shifted(win[i], win[i + 1], shift), x, T());
+#pragma unroll
+                            for (int q = 0; q < E; ++q) x[q] = ex2((x[q] - f.m) * c) * fac;
+                        }
+                        dst[i] = pack(x, T());
+                    }
+                    arrive(&sh.empty[st]);
+                }
+                // logits before the first and after the last of those slots: by element
+                const int j0 = max(base, 0), j1 = min(base + sl.m * E, a.v);
+                const int ja = sl.w1 > sl.w0 ? slot_at(base + sl.w0 * E) * E - lead : j1, jb = sl.w1 > sl.w0 ? (end + lead) / E * E - lead : j1;
+                if (tid < 4 * E) {
+                    const int j = tid < 2 * E ? j0 + tid : max(jb, ja) + tid - 2 * E;
+                    if (j < (tid < 2 * E ? min(ja, j1) : j1)) o[j] = from_f<T>(zero ? 0.f : ex2((to_f(__ldg(row.p + j)) - f.m) * c) * fac);
+                }
+                if (!zero) {
+                    rows_sync<CT>();        // the dense gradient lies before the teacher's places
+                    if (tid < a.k) {
+                        const int id = teach.id[tid];
+                        if (id >= j0 && id < j1) {
+                            float q = 0.f;
+                            for (int i = 0; i < a.k; ++i) q += teach.id[i] == id ? teach.q[i] : 0.f;
+                            o[id] = from_f<T>(ex2((teach.z[tid] - f.m) * c) * fac - up * q);
+                        }
+                    }
+                }
+            }
+        }
+        arrive(&sh.side_empty[b]);
     }
 }
 
@@ -771,7 +978,7 @@ template <int L> __device__ __forceinline__ float lanes_sum(float x) {
 }
 
 template <class T, int L, int E, int MODE>
-__global__ void __launch_bounds__(TT) token_lanes_kernel(LanesArgs a) {
+__global__ void __launch_bounds__(TT) token_lanes_kernel(const LanesArgs a) {
     extern __shared__ __align__(16) unsigned char dyn[];
     const long long want = ((long long)blockIdx.x * TT + threadIdx.x) / L;
     const bool live = want < a.rows;
@@ -909,11 +1116,13 @@ __global__ void __launch_bounds__(TT) token_lanes_kernel(LanesArgs a) {
 
 // ---- launches --------------------------------------------------------------------------------------
 
-template <class K, class... A>
-int launch_rows(Device* dev, K kernel, long long blocks, int cluster, size_t smem, A... args) {
+template <class T> constexpr int dtype_slot() { return std::is_same<T, float>::value ? 0 : std::is_same<T, __half>::value ? 1 : 2; }
+
+template <class A>
+int launch_rows(Device* dev, void (*kernel)(A), long long blocks, int cluster, size_t smem, const A& args, int threads = TT) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(TT);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = dev->stream;
     cudaLaunchAttribute attr[1];
@@ -921,9 +1130,43 @@ int launch_rows(Device* dev, K kernel, long long blocks, int cluster, size_t sme
     attr[0].val.clusterDim.x = (unsigned)cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
-    EB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    EB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, args));
     count_launch();
     return EB200_OK;
+}
+
+template <class T, int MODE>
+int launch_rows_of(Device* dev, const TokenShape& t, const RowsArgs& a) {
+    using S = RowsShape<MODE>;
+    if (!(dev->token_configured >> (MODE * 3 + dtype_slot<T>()) & 1)) {
+        EB_CHECK_CUDA(cudaFuncSetAttribute(token_rows_kernel<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(RowsShared<MODE>)));
+        dev->token_configured |= 1u << (MODE * 3 + dtype_slot<T>());
+    }
+    const long long ctas = t.cluster > 1 ? t.n * t.cluster : std::min(t.n, (long long)dev->prop.multiProcessorCount * S::CTAS);
+    return launch_rows(dev, token_rows_kernel<T, MODE>, ctas, t.cluster, sizeof(RowsShared<MODE>), a, S::THREADS);
+}
+
+template <class T>
+int launch_long(Device* dev, const Plan& plan, const void* const* in, void* const* out) {
+    const TokenShape& t = plan.tok;
+    const int wide = t.id_dtype == EB200_I64, esize = wide ? 8 : 4;
+    auto index = [&](int i) { return (const void*)(reinterpret_cast<const char*>(in[i]) + plan.p.in[i].offset * esize); };
+    RowsArgs a = {};
+    a.z = reinterpret_cast<const T*>(in[0]) + t.offset;
+    a.pitch = t.pitch; a.g_pitch = t.g_pitch; a.rows = t.n; a.v = t.v; a.k = t.k; a.scale = t.scale; a.wide = wide;
+    a.cluster = t.cluster; a.per = t.slice; a.error_flag = dev->error_flag_dev;
+    if (plan.impl == IMPL_TOKEN_LOGPROB) {
+        a.ids = index(1);
+        a.out = {reinterpret_cast<float*>(out[0]) + t.g_offset, reinterpret_cast<float*>(out[1]), reinterpret_cast<float*>(out[2]),
+                 t.k ? reinterpret_cast<float*>(out[3]) : nullptr, t.k ? reinterpret_cast<int*>(out[4]) : nullptr};
+        return t.k ? launch_rows_of<T, ROWS_TOP>(dev, t, a) : launch_rows_of<T, ROWS_LOGPROB>(dev, t, a);
+    }
+    a.te = {reinterpret_cast<const char*>(in[1]) + plan.p.in[1].offset * (t.teacher_dtype == EB200_F32 ? 4 : 2), index(2), t.teacher_dtype, wide};
+    a.loss = reinterpret_cast<float*>(out[0]) + (t.grad ? 0 : t.g_offset);
+    if (!t.grad) return launch_rows_of<T, ROWS_DISTILL>(dev, t, a);
+    a.weights = reinterpret_cast<const float*>(in[3]) + plan.p.in[3].offset;
+    a.g = reinterpret_cast<T*>(out[1]) + t.g_offset;
+    return launch_rows_of<T, ROWS_DISTILL_GRAD>(dev, t, a);
 }
 
 template <class T, int L, int E>
@@ -970,54 +1213,51 @@ int launch_lanes(Device* dev, const Plan& plan, const void* const* in, void* con
 }
 
 template <class T>
-int launch_typed(Device* dev, const Plan& plan, const void* const* in, void* const* out) {
+int launch_grad(Device* dev, const Plan& plan, const void* const* in, void* const* out) {
     const TokenShape& t = plan.tok;
-    if (t.lanes) return launch_lanes<T>(dev, plan, in, out);
-    const T* z = reinterpret_cast<const T*>(in[0]) + t.offset;
     const int wide = t.id_dtype == EB200_I64, esize = wide ? 8 : 4;
     auto vec = [&](int i) { return reinterpret_cast<const float*>(in[i]) + plan.p.in[i].offset; };
-    auto index = [&](int i) { return (const void*)(reinterpret_cast<const char*>(in[i]) + plan.p.in[i].offset * esize); };
-    if (plan.impl == IMPL_TOKEN_LOGPROB) {
-        LogprobOut o = {reinterpret_cast<float*>(out[0]) + t.g_offset, reinterpret_cast<float*>(out[1]), reinterpret_cast<float*>(out[2]),
-                        t.k ? reinterpret_cast<float*>(out[3]) : nullptr, t.k ? reinterpret_cast<int*>(out[4]) : nullptr};
-        if (t.k) return launch_rows(dev, token_logprob_kernel<T, true>, t.n * t.cluster, t.cluster, sizeof(TopShared), z, t.pitch, t.v, t.k, t.scale, index(1), wide, o, t.cluster);
-        return launch_rows(dev, token_logprob_kernel<T, false>, t.n * t.cluster, t.cluster, 0, z, t.pitch, t.v, t.k, t.scale, index(1), wide, o, t.cluster);
-    }
-    if (plan.impl == IMPL_TOKEN_LOGPROB_GRAD) {
-        T* g = reinterpret_cast<T*>(out[0]) + t.g_offset;
-        constexpr int E = Pack<T>::E;
-        const int per_row = (t.v + E - 1 + E - 1) / E / (32 * GU) + 1;
-        const long long blocks = (t.n * per_row + NW - 1) / NW;
-        EB_REQUIRE(blocks < (1LL << 31), EB200_ERR_UNSUPPORTED, "token log-probability gradient over %lld rows of %d", t.n, t.v);
-        if (t.entropy) return launch_rows(dev, token_logprob_grad_kernel<T, true>, blocks, 1, 0, z, t.pitch, g, t.g_pitch, t.n, t.v, t.scale, index(1), wide, vec(2), vec(3), vec(4), vec(5), per_row);
-        return launch_rows(dev, token_logprob_grad_kernel<T, false>, blocks, 1, 0, z, t.pitch, g, t.g_pitch, t.n, t.v, t.scale, index(1), wide, vec(2), vec(3), (const float*)nullptr, (const float*)nullptr, per_row);
-    }
-    const int vsize = t.teacher_dtype == EB200_F32 ? 4 : 2;
-    const Teacher te = {reinterpret_cast<const char*>(in[1]) + plan.p.in[1].offset * vsize, index(2), t.teacher_dtype, wide};
-    float* loss = reinterpret_cast<float*>(out[0]) + (t.grad ? 0 : t.g_offset);
-    if (t.grad)
-        return launch_rows(dev, distill_topk_kernel<T, true>, t.n * t.cluster, t.cluster, 0, z, t.pitch, t.v, t.k, t.scale, te, vec(3), loss,
-                           reinterpret_cast<T*>(out[1]) + t.g_offset, t.g_pitch, t.cluster);
-    return launch_rows(dev, distill_topk_kernel<T, false>, t.n * t.cluster, t.cluster, 0, z, t.pitch, t.v, t.k, t.scale, te, (const float*)nullptr, loss, (T*)nullptr, 0LL, t.cluster);
+    constexpr int E = Pack<T>::E;
+    GradArgs a = {};
+    a.z = reinterpret_cast<const T*>(in[0]) + t.offset;
+    a.g = reinterpret_cast<T*>(out[0]) + t.g_offset;
+    a.pitch = t.pitch; a.g_pitch = t.g_pitch; a.rows = t.n; a.v = t.v; a.scale = t.scale; a.wide = wide;
+    a.ids = reinterpret_cast<const char*>(in[1]) + plan.p.in[1].offset * esize;
+    a.lse = vec(2); a.g_logp = vec(3);
+    if (t.entropy) { a.entropy = vec(4); a.g_entropy = vec(5); }
+    a.per_row = (t.v + 2 * (E - 1)) / E / (32 * GU) + 1;
+    const long long blocks = (t.n * a.per_row + NW - 1) / NW;
+    EB_REQUIRE(blocks < (1LL << 31), EB200_ERR_UNSUPPORTED, "token log-probability gradient over %lld rows of %d", t.n, t.v);
+    return t.entropy ? launch_rows(dev, token_logprob_grad_kernel<T, true>, blocks, 1, 0, a) : launch_rows(dev, token_logprob_grad_kernel<T, false>, blocks, 1, 0, a);
+}
+
+template <class T>
+int launch_typed(Device* dev, const Plan& plan, const void* const* in, void* const* out) {
+    if (plan.tok.lanes) return launch_lanes<T>(dev, plan, in, out);
+    return plan.impl == IMPL_TOKEN_LOGPROB_GRAD ? launch_grad<T>(dev, plan, in, out) : launch_long<T>(dev, plan, in, out);
 }
 
 }  // namespace
 
 // Short rows in registers: 4 lanes up to 16 logits, 8 up to 64, a warp up to 256 (the gradient) or 1024 (the rest).
 // A distillation's teacher entries lie in shared memory, so many entries per row want more lanes.
-// Few longer rows: the CTAs of a cluster share one, until the GPU is full or a CTA has less than two slots per thread.
+// Few longer rows: the CTAs of a cluster share one, until the GPU is full or a slice has less than two slots per thread.
 void token_variant(TokenShape* t, int sm_count) {
     t->cluster = 1;
     t->lanes = 0;
-    const bool logprob_grad = t->grad && t->k == 0;
+    t->slice = 0;
+    const bool logprob_grad = t->grad && !t->distill;
     if (t->v <= (logprob_grad ? 256 : 1024)) {
         t->lanes = t->v <= 16 ? 4 : t->v <= 64 ? 8 : 32;
         while (t->lanes < 32 && TT / t->lanes * t->k * 12 > 32768) t->lanes = t->lanes == 4 ? 8 : 32;
         return;
     }
     if (logprob_grad) return;
-    const long long slots = (long long)t->v / (t->dtype == EB200_F32 ? 4 : 8);
-    while (t->cluster < MAX_CLUSTER && t->n * t->cluster * 2 <= 2LL * sm_count && slots / (t->cluster * 2) >= 2 * TT) t->cluster *= 2;
+    const int e = t->dtype == EB200_F32 ? 4 : 8;
+    const long long slots = ((long long)t->v + 2 * (e - 1)) / e;       // at the worst alignment
+    const long long ctas = (long long)sm_count * (t->grad ? RowsShape<ROWS_DISTILL_GRAD>::CTAS : RowsShape<ROWS_LOGPROB>::CTAS);
+    while (t->cluster < MAX_CLUSTER && t->n * t->cluster * 2 <= ctas && slots / (t->cluster * 2) >= 2 * TT) t->cluster *= 2;
+    t->slice = (int)((slots + t->cluster - 1) / t->cluster);
 }
 
 int launch_token(Device* dev, const Plan& plan, const void* const* in, void* const* out) {
