@@ -111,9 +111,11 @@ template <class T> struct Row {
 // reference and count as 0; a row whose maximum lies beyond NEAR / c is summed again against that maximum.
 constexpr float NEAR = 4194304.f, FAR = 8388608.f;
 
+typedef unsigned long long f32x2;
+
 struct Acc {
     float rc = 0.f, lim, mx = NEG_INF;
-    float2 s = {0.f, 0.f}, t = {0.f, 0.f};
+    f32x2 s = 0, t = 0;                                   // two sums each, of even and odd places
     int slot = -1;
     __device__ __forceinline__ explicit Acc(float c) : lim(-FAR / c) {}
 };
@@ -121,24 +123,18 @@ struct Acc {
 // y of a logit far below its reference counts as -1000: e is 0 there and e * y must not be 0 * inf
 __device__ __forceinline__ float floor_y(float y) { return fmaxf(y, -1000.f); }
 
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{ .reg .b64 a, b, c, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7}; fma.rn.f32x2 d, a, b, c; mov.b64 {%0, %1}, d; }"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("{ .reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; add.rn.f32x2 d, a, b; mov.b64 {%0, %1}, d; }"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
+// two f32 in a 64-bit register
+__device__ __forceinline__ f32x2 pair(float lo, float hi) { f32x2 d; asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi)); return d; }
+__device__ __forceinline__ float2 parts(f32x2 a) { float2 d; asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(a)); return d; }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { f32x2 d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
 
 __device__ __forceinline__ void move_reference(Acc& a, float mx, float c) {
     const float rc = fminf(rintf(mx * c), FAR);
     const float dy = fminf(floor_y(a.rc - rc), 0.f), f = ex2(dy);       // 0 sums before the first reference
-    a.t.x = f * fmaf(dy, a.s.x, a.t.x); a.t.y = f * fmaf(dy, a.s.y, a.t.y);
-    a.s.x *= f; a.s.y *= f;
+    const f32x2 ff = pair(f, f);
+    a.t = fma2(ff, fma2(pair(dy, dy), a.s, a.t), 0);
+    a.s = fma2(ff, a.s, 0);
     a.rc = rc;
     a.lim = (rc + HEADROOM) / c;
 }
@@ -147,6 +143,8 @@ __device__ __forceinline__ void move_reference(Acc& a, float mx, float c) {
 // -inf becomes a finite value whose e is 0 (`low`; NaN stays).
 template <class T> struct Bits;
 template <> struct Bits<float> {
+    static __device__ __forceinline__ unsigned more(unsigned a, unsigned b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+    static __device__ __forceinline__ uint4 larger(const uint4& a, const uint4& b) { return make_uint4(more(a.x, b.x), more(a.y, b.y), more(a.z, b.z), more(a.w, b.w)); }
     static __device__ __forceinline__ float largest(const uint4& u) {
         return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
     }
@@ -162,6 +160,8 @@ template <> struct Bits<float> {
 };
 template <> struct Bits<__nv_bfloat16> {
     static __device__ __forceinline__ __nv_bfloat162 as(unsigned w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
+    static __device__ __forceinline__ unsigned more(unsigned a, unsigned b) { const __nv_bfloat162 m = __hmax2(as(a), as(b)); return *reinterpret_cast<const unsigned*>(&m); }
+    static __device__ __forceinline__ uint4 larger(const uint4& a, const uint4& b) { return make_uint4(more(a.x, b.x), more(a.y, b.y), more(a.z, b.z), more(a.w, b.w)); }
     static __device__ __forceinline__ float largest(const uint4& u) {
         const __nv_bfloat162 m = __hmax2(__hmax2(as(u.x), as(u.y)), __hmax2(as(u.z), as(u.w)));
         return fmaxf(__low2float(m), __high2float(m));
@@ -178,6 +178,8 @@ template <> struct Bits<__nv_bfloat16> {
 };
 template <> struct Bits<__half> {
     static __device__ __forceinline__ __half2 as(unsigned w) { return *reinterpret_cast<__half2*>(&w); }
+    static __device__ __forceinline__ unsigned more(unsigned a, unsigned b) { const __half2 m = __hmax2(as(a), as(b)); return *reinterpret_cast<const unsigned*>(&m); }
+    static __device__ __forceinline__ uint4 larger(const uint4& a, const uint4& b) { return make_uint4(more(a.x, b.x), more(a.y, b.y), more(a.z, b.z), more(a.w, b.w)); }
     static __device__ __forceinline__ float largest(const uint4& u) {
         const __half2 m = __hmax2(__hmax2(as(u.x), as(u.y)), __hmax2(as(u.z), as(u.w)));
         return fmaxf(__low2float(m), __high2float(m));
@@ -191,9 +193,10 @@ template <> struct Bits<__half> {
 };
 
 template <bool ENT>
-__device__ __forceinline__ void add_pair(Acc& a, float2 x, float c) {
-    const float2 y = fma2(x, make_float2(c, c), make_float2(-a.rc, -a.rc));
-    const float2 e = make_float2(ex2(y.x), ex2(y.y));
+__device__ __forceinline__ void add_pair(Acc& a, float2 x, f32x2 c, f32x2 minus_rc) {
+    const f32x2 y = fma2(pair(x.x, x.y), c, minus_rc);
+    const float2 p = parts(y);
+    const f32x2 e = pair(ex2(p.x), ex2(p.y));
     a.s = add2(a.s, e);
     if (ENT) a.t = fma2(e, y, a.t);
 }
@@ -202,22 +205,28 @@ __device__ __forceinline__ void add_pair(Acc& a, float2 x, float c) {
 template <class T, bool ENT, bool TOP, int N>
 __device__ __forceinline__ void take(Acc& a, const uint4 (&u)[N], int slot, int step, float c) {
     float mx = NEG_INF;
+    if (TOP) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float m = Bits<T>::largest(u[i]);
-        if (TOP) {
+        for (int i = 0; i < N; ++i) {
+            const float m = Bits<T>::largest(u[i]);
             if (m > a.mx) { a.mx = m; a.slot = slot + i * step; }
+            mx = fmaxf(mx, m);
         }
-        mx = fmaxf(mx, m);
+    } else {
+        uint4 m = u[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) m = Bits<T>::larger(m, u[i]);
+        mx = fmaxf(mx, Bits<T>::largest(m));
+        a.mx = fmaxf(a.mx, mx);
     }
-    if (!TOP) a.mx = fmaxf(a.mx, mx);
     if (mx > a.lim) move_reference(a, mx, c);
+    const f32x2 cc = pair(c, c), minus_rc = pair(-a.rc, -a.rc);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         float2 x[Pack<T>::E / 2];
         Bits<T>::template pairs<ENT>(u[i], x, c);
 #pragma unroll
-        for (int q = 0; q < Pack<T>::E / 2; ++q) add_pair<ENT>(a, x[q], c);
+        for (int q = 0; q < Pack<T>::E / 2; ++q) add_pair<ENT>(a, x[q], cc, minus_rc);
     }
 }
 
@@ -233,8 +242,8 @@ __device__ __forceinline__ void take_part(Acc& a, const float (&x)[Pack<T>::E], 
 #pragma unroll
     for (int i = 0; i < Pack<T>::E; ++i) {
         const float y = fmaf(x[i], c, -a.rc), e = ex2(y);
-        a.s.x += e;
-        if (ENT) a.t.x = fmaf(e, floor_y(y), a.t.x);
+        a.s = add2(a.s, pair(e, 0.f));
+        if (ENT) a.t = add2(a.t, pair(e * floor_y(y), 0.f));
     }
 }
 
@@ -258,8 +267,9 @@ template <int CT> __device__ __forceinline__ void rows_sync() { asm volatile("ba
 // the CTA's totals on all those threads, joined in the same order everywhere
 template <int CT>
 __device__ __forceinline__ Stat cta_totals(const Acc& a, StatShared<CT>& sh) {
-    const float s = a.s.x + a.s.y;
-    Stat st = {s == 0.f ? -2.f * FAR : a.rc, s, a.t.x + a.t.y, a.mx};
+    const float2 sp = parts(a.s), tp = parts(a.t);
+    const float s = sp.x + sp.y;
+    Stat st = {s == 0.f ? -2.f * FAR : a.rc, s, tp.x + tp.y, a.mx};
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) {
         Stat q;
@@ -333,8 +343,8 @@ template <bool ENT, int E> __device__ __forceinline__ void take_against(Acc& b, 
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         const float y = (x[i] - m) * c, e = ex2(y);
-        b.s.x += e;
-        if (ENT) b.t.x = fmaf(e, floor_y(y), b.t.x);
+        b.s = add2(b.s, pair(e, 0.f));
+        if (ENT) b.t = add2(b.t, pair(e * floor_y(y), 0.f));
     }
 }
 __device__ __forceinline__ Final finish_against(const Stat& st, float m) { return {m, st.s, logf(st.s), LN2 * (st.t / st.s), false}; }
@@ -487,32 +497,19 @@ __device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int shi
     return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
 }
 
-// logits [j, j + E) of a row that starts at p: the aligned 16 bytes around them, as long as those lie inside the row
-template <class T> struct Window {
-    static constexpr int E = Pack<T>::E;
-    uint4 a, b;
-    float x[E];
-    int kind;        // 0 aligned, 1 shifted, 2 element by element
-    __device__ __forceinline__ void load(const T* p, int v, int j, int shift) {
-        const int down = shift / (int)sizeof(T);
-        const uint4* at = reinterpret_cast<const uint4*>(p + j - down);
-        if (shift == 0 && j >= 0 && j + E <= v) { kind = 0; a = __ldg(at); }
-        else if (shift != 0 && j - down >= 0 && j - down + 2 * E <= v) { kind = 1; a = __ldg(at); b = __ldg(at + 1); }
-        else {
-            kind = 2;
+// logits [j, j + E) of a row of v that starts at p, element by element where the 16 aligned bytes around them (two times
+// 16 if `shift`, the bytes by which p + j lies beyond a boundary) leave the row
+template <class T> __device__ __forceinline__ void window(const T* p, int v, int j, int shift, float (&x)[Pack<T>::E]) {
+    constexpr int E = Pack<T>::E;
+    const int down = shift / (int)sizeof(T);
+    const uint4* at = reinterpret_cast<const uint4*>(p + j - down);
+    if (shift == 0 && j >= 0 && j + E <= v) unpack(__ldg(at), x, T());
+    else if (shift != 0 && j - down >= 0 && j - down + 2 * E <= v) unpack(shifted(__ldg(at), __ldg(at + 1), shift), x, T());
+    else {
 #pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = j + i >= 0 && j + i < v ? to_f(__ldg(p + j + i)) : NEG_INF;
-        }
+        for (int i = 0; i < E; ++i) x[i] = j + i >= 0 && j + i < v ? to_f(__ldg(p + j + i)) : NEG_INF;
     }
-    __device__ __forceinline__ void get(float (&y)[E], int shift) {
-        if (kind == 2) {
-#pragma unroll
-            for (int i = 0; i < E; ++i) y[i] = x[i];
-        } else {
-            unpack(kind == 0 ? a : shifted(a, b, shift), y, T());
-        }
-    }
-};
+}
 
 template <class T> __device__ __forceinline__ void put(T* p, int v, int j, const float (&y)[Pack<T>::E]) {
     constexpr int E = Pack<T>::E;
@@ -528,7 +525,7 @@ template <class T> __device__ __forceinline__ void put(T* p, int v, int j, const
 // ---- gradient --------------------------------------------------------------------------------------
 // d_j = scale * (g_l ([j = t] - p_j) - g_H p_j (ln p_j + H)), p_j = exp(x_j - lse): a stream of logits in and a
 // stream of gradients out, cut along 16-byte slots of the output so that stores stay whole whatever the pitches.
-// A warp takes 32 * GU slots of a row.
+// A CTA takes GU * 256 slots of a row; all of them whole is the rule, and then nothing is tested per slot.
 constexpr int GU = 4;
 
 struct GradArgs {
@@ -543,50 +540,68 @@ struct GradArgs {
 };
 
 template <class T, bool ENT>
-__global__ void __launch_bounds__(TT) token_logprob_grad_kernel(const GradArgs a) {
+__global__ void __launch_bounds__(TT, 5) token_logprob_grad_kernel(const GradArgs a) {
     constexpr int E = Pack<T>::E;
-    const int per_row = a.per_row, v = a.v;
-    const float scale = a.scale;
-    const long long task = (long long)blockIdx.x * NW + (threadIdx.x >> 5);
-    const long long n = task / per_row;
-    if (n >= a.rows) return;
-    const int lane = threadIdx.x & 31, s0 = (int)(task % per_row) * 32 * GU + lane;
+    const int v = a.v, tid = threadIdx.x;
+    const long long n = blockIdx.x / a.per_row;
+    const int s0 = (int)(blockIdx.x % a.per_row) * GU * TT + tid;
     const T* p = reinterpret_cast<const T*>(a.z) + n * a.pitch;
     T* o = reinterpret_cast<T*>(a.g) + n * a.g_pitch;
-    const int lead = (int)((reinterpret_cast<uintptr_t>(o) & 15) / sizeof(T));
-    const int slots = (lead + v + E - 1) / E;
-    const int shift = (int)(reinterpret_cast<uintptr_t>(p - lead) & 15);
     const long long t = load_id(a.ids, n, a.wide);
     const float norm = __ldg(a.lse + n), gl = t >= 0 && t < v ? __ldg(a.g_logp + n) : 0.f;
     const float gh = ENT ? __ldg(a.g_entropy + n) : 0.f, h = ENT ? __ldg(a.entropy + n) : 0.f;
+    const int lead = (int)((reinterpret_cast<uintptr_t>(o) & 15) / sizeof(T));
+    const int slots = (lead + v + E - 1) / E;
+    const int shift = (int)(reinterpret_cast<uintptr_t>(p - lead) & 15);
     const bool zero = norm == NEG_INF || (gl == 0.f && gh == 0.f);
-    const float up = gl * scale, al = -up, ah = -gh * scale;
-    Window<T> w[GU];
-    if (!zero) {
+    const float up = gl * a.scale, ah = -gh * a.scale;
+
+    auto gradient = [&](float (&x)[E], int s) {
 #pragma unroll
-        for (int i = 0; i < GU; ++i)
-            if (s0 + i * 32 < slots) w[i].load(p, v, (s0 + i * 32) * E - lead, shift);
+        for (int q = 0; q < E; ++q) {
+            const float d = fmaf(x[q], a.scale, -norm), pr = ex2(d * LOG2E);
+            x[q] = pr * (ENT ? fmaf(ah, floor_y(d) + h, -up) : -up);
+        }
+        const long long at = t - ((long long)s * E - lead);
+        if (at >= 0 && at < E) {
+#pragma unroll
+            for (int q = 0; q < E; ++q) x[q] += q == (int)at ? up : 0.f;
+        }
+    };
+
+    const int lo = s0 - tid, hi = lo + GU * TT;
+    if (!zero && lo * E - lead - (shift ? E : 0) >= 0 && (hi + (shift ? 1 : 0)) * E - lead <= v) {
+        const uint4* from = reinterpret_cast<const uint4*>(p - lead - shift / (int)sizeof(T)) + s0;
+        uint4* to = reinterpret_cast<uint4*>(o - lead) + s0;
+        uint4 u[GU];
+        if (shift == 0) {
+#pragma unroll
+            for (int i = 0; i < GU; ++i) u[i] = __ldcs(from + i * TT);
+        } else {
+            uint4 w[GU];
+#pragma unroll
+            for (int i = 0; i < GU; ++i) { u[i] = __ldg(from + i * TT); w[i] = __ldg(from + i * TT + 1); }
+#pragma unroll
+            for (int i = 0; i < GU; ++i) u[i] = shifted(u[i], w[i], shift);
+        }
+#pragma unroll
+        for (int i = 0; i < GU; ++i) {
+            float x[E];
+            unpack(u[i], x, T());
+            gradient(x, s0 + i * TT);
+            __stcs(to + i * TT, pack(x, T()));
+        }
+        return;
     }
-#pragma unroll
-    for (int i = 0; i < GU; ++i) {
-        const int s = s0 + i * 32, j = s * E - lead;
-        if (s >= slots) break;
+    for (int s = s0; s < min(hi, slots); s += TT) {
+        const int j = s * E - lead;
         float x[E];
         if (zero) {
 #pragma unroll
             for (int q = 0; q < E; ++q) x[q] = 0.f;
         } else {
-            w[i].get(x, shift);
-#pragma unroll
-            for (int q = 0; q < E; ++q) {
-                const float d = fmaf(x[q], scale, -norm), pr = ex2(d * LOG2E);
-                x[q] = pr * (ENT ? fmaf(ah, floor_y(d) + h, al) : al);
-            }
-            const long long at = t - j;
-            if (at >= 0 && at < E) {
-#pragma unroll
-                for (int q = 0; q < E; ++q) x[q] += q == (int)at ? up : 0.f;
-            }
+            window(p, v, j, shift, x);
+            gradient(x, s);
         }
         put(o, v, j, x);
     }
@@ -1225,8 +1240,8 @@ int launch_grad(Device* dev, const Plan& plan, const void* const* in, void* cons
     a.ids = reinterpret_cast<const char*>(in[1]) + plan.p.in[1].offset * esize;
     a.lse = vec(2); a.g_logp = vec(3);
     if (t.entropy) { a.entropy = vec(4); a.g_entropy = vec(5); }
-    a.per_row = (t.v + 2 * (E - 1)) / E / (32 * GU) + 1;
-    const long long blocks = (t.n * a.per_row + NW - 1) / NW;
+    a.per_row = (int)(((t.v + 2LL * (E - 1)) / E + GU * TT - 1) / (GU * TT));       // at the worst alignment
+    const long long blocks = t.n * a.per_row;
     EB_REQUIRE(blocks < (1LL << 31), EB200_ERR_UNSUPPORTED, "token log-probability gradient over %lld rows of %d", t.n, t.v);
     return t.entropy ? launch_rows(dev, token_logprob_grad_kernel<T, true>, blocks, 1, 0, a) : launch_rows(dev, token_logprob_grad_kernel<T, false>, blocks, 1, 0, a);
 }
