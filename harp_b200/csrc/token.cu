@@ -22,7 +22,6 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int TT = 256;                     // threads per CTA
-constexpr int NW = TT / 32;
 constexpr int MAX_CLUSTER = 8;
 constexpr int MAX_K = 64;                   // alternatives
 constexpr int GROUPS = 64;                  // groups of threads whose maxima bound the k-th largest logit, >= MAX_K
@@ -994,7 +993,7 @@ template <int L> __device__ __forceinline__ float lanes_sum(float x) {
 
 template <class T, int L, int E, int MODE>
 __global__ void __launch_bounds__(TT) token_lanes_kernel(const LanesArgs a) {
-    extern __shared__ __align__(16) unsigned char dyn[];
+    extern __shared__ __align__(128) unsigned char dyn[];
     const long long want = ((long long)blockIdx.x * TT + threadIdx.x) / L;
     const bool live = want < a.rows;
     const long long n = live ? want : a.rows - 1;          // lanes without a row follow the last one and store nothing
