@@ -316,18 +316,24 @@ __device__ __forceinline__ Stat exchange(const Stat& mine, StatShared<CT>& sh, u
     return st;
 }
 
-// against the row's maximum m: S >= 1, ln S, and mean = sum e (x - m) / S.  A row of -inf is `empty`.
+// against the row's maximum m: S >= 1, ln S >= 0, and mean = sum e (x - m) / S <= 0.  A row of -inf is `empty`.
 struct Final { float m, s, ln_s, mean; bool empty; };
 
+// The largest logit's own terms, rounded here as they were when they were added, come off both sums first: what the
+// others leave is 0 for a row of one possible logit, so its ln S and its entropy are exactly 0, and no rounding can make
+// a probability larger than 1 or an entropy negative.  (s * 2^-dy, two roundings, gave S < 1 on every fifth such row.)
 __device__ __forceinline__ Final finish(const Stat& st, float c) {
     Final f;
     f.m = st.mx;
     f.empty = st.mx == NEG_INF && st.s == 0.f;                  // a NaN makes s NaN
     if (f.empty) { f.s = 1.f; f.ln_s = 0.f; f.mean = 0.f; return f; }
-    const float dy = fmaf(st.mx, c, -st.rc);
-    f.s = st.s * ex2(-dy);
-    f.ln_s = logf(f.s);
-    f.mean = LN2 * (st.t / st.s - dy);
+    const float dy = fmaf(st.mx, c, -st.rc), own = ex2(dy), rest = st.s - own;
+    float others = rest / own, mean = LN2 * (fmaf(-dy, rest, st.t - __fmul_rn(own, dy)) / st.s);
+    if (others < 0.f) others = 0.f;                             // NaN stays
+    if (mean > 0.f) mean = 0.f;
+    f.s = 1.f + others;
+    f.ln_s = log1pf(others);
+    f.mean = mean;
     return f;
 }
 

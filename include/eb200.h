@@ -114,7 +114,8 @@ typedef enum {
                               * for K > 0 the log-probabilities [N, K] F32 and indices [N, K] I32 of the K largest logits, largest
                               * first, equal ones by the lowest index.  A token outside [0, V) marks padding: its logp is 0, the
                               * rest of the row's outputs do not depend on it.  -inf logits have probability 0; a row of nothing
-                              * else has logp, lse and alternatives -inf and entropy 0.  A row that holds a NaN or +inf has NaN in
+                              * else has logp, lse and alternatives -inf and entropy 0.  Log-probabilities are never above 0, entropies
+                              * never below; a row of one possible token has exactly 0 for both.  A row that holds a NaN or +inf has NaN in
                               * its float outputs; NaN ranks like -inf among the alternatives.
                               * Gradient (flags bit 7): inputs logits, tokens, lse [N], g_logp [N] and, with an entropy term,
                               * entropy [N] and g_entropy [N] (lse and entropy as the forward kernel left them); output [N, V] in

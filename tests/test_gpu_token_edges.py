@@ -204,3 +204,33 @@ def test_nan_in_the_token_gradient(dev, registry, kind, n, v):
         want, tol = R.logprob_grad(z[plain], ids[plain], lse[plain], np.where(ids < 0, 0, gl)[plain], h[plain] if entropy else None,
                                    gh[plain] if entropy else None, 1.0, kind)
         near(got[plain], want, tol, f"entropy {entropy}")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,v,k", [(64, 1000, 3), (64, 1025, 3), (700, 2500, 0), (700, 2500, 3), (200, 5003, 0), (6, 131072, 3), (6, 131072, 0)])
+def test_a_certain_token_has_probability_one(dev, registry, kind, n, v, k):
+    """Rows with one possible token (a grammar's forced one): log-probability, entropy and loss are exactly 0, whatever the
+    length, since nothing is added to the token's own exponential.  Rows where another token is all but impossible:
+    probabilities stay at 1 or below and entropies at 0 or above."""
+    rng = np.random.default_rng(v)
+    x = np.full((n, v), -np.inf, np.float32)
+    ids = rng.integers(0, v, n)
+    x[np.arange(n), ids] = rng.uniform(-30, 30, n)
+    x[1::2] = logits(rng, (n + 1) // 2, v)[:n // 2]
+    x[1::2][np.arange(n // 2), ids[1::2]] = rng.uniform(40, 70, n // 2)
+    stored, z = store(x, kind)
+    got, kern = run_logprob(dev, registry, stored, ids, k, kind, 0.9, v + 1, 3)
+    one = slice(0, None, 2)
+    assert (got["logp"][one] == 0).all(), (kern.impl, got["logp"][one].min(), got["logp"][one].max())
+    assert (got["entropy"][one] == 0).all(), (kern.impl, got["entropy"][one].min(), got["entropy"][one].max())
+    assert (got["logp"] <= 0).all() and (got["entropy"] >= 0).all(), kern.impl
+    if k:
+        assert (got["top_ids"][:, 0] == ids).all()
+        assert (got["top"][one, 0] == 0).all() and np.isneginf(got["top"][one, 1:]).all() and (got["top"] <= 0).all()
+    ref, tol = R.logprob(z, ids, k, 0.9)
+    for key in tol:
+        near(got[key], ref[key], tol[key], f"{key} {kern.impl}")
+    loss, loss2, grad, kerns = run_distill(dev, registry, stored, np.zeros((n, 1), np.float32), ids[:, None].astype(np.int32), np.ones(n, np.float32), kind,
+                                           "f32", 0.9, v + 1, 3)
+    assert (loss[one] == 0).all() and (loss2[one] == 0).all() and (loss >= 0).all() and (loss2 >= 0).all(), kerns[0].impl
+    assert (grad[one] == 0).all(), kerns[1].impl
