@@ -534,6 +534,10 @@ template <class T> __device__ __forceinline__ void put(T* p, int v, int j, const
 // it: 4096 x 131072 bf16 with the entropy's term takes 359 us, 5.98 TB/s (a warp per 128 slots with tests per slot: 513).
 constexpr int GU = 4;
 
+// lse in f32 is off by up to a quarter from here on (rows of a mask's lowest value, logits of millions): x_j - lse may then
+// round far above 0, and is held at 0, so that p_j stays a probability.  Below, p_j is off by what lse's rounding makes it.
+constexpr float FAR_LSE = 4194304.f;
+
 struct GradArgs {
     const void* z;
     void* g;
@@ -559,13 +563,15 @@ __global__ void __launch_bounds__(TT, 5) token_logprob_grad_kernel(const GradArg
     const int lead = (int)((reinterpret_cast<uintptr_t>(o) & 15) / sizeof(T));
     const int slots = (lead + v + E - 1) / E;
     const int shift = (int)(reinterpret_cast<uintptr_t>(p - lead) & 15);
-    const bool zero = norm == NEG_INF || (gl == 0.f && gh == 0.f);
+    const bool zero = norm == NEG_INF || (gl == 0.f && gh == 0.f), far = fabsf(norm) >= FAR_LSE;
     const float up = gl * a.scale, ah = -gh * a.scale;
 
-    auto gradient = [&](float (&x)[E], int s) {
+    auto gradient = [&](float (&x)[E], int s, bool hold) {
 #pragma unroll
         for (int q = 0; q < E; ++q) {
-            const float d = fmaf(x[q], a.scale, -norm), pr = ex2(d * LOG2E);
+            float d = fmaf(x[q], a.scale, -norm);
+            if (hold && d > 0.f) d = 0.f;
+            const float pr = ex2(d * LOG2E);
             x[q] = pr * (ENT ? fmaf(ah, floor_y(d) + h, -up) : -up);
         }
         const long long at = t - ((long long)s * E - lead);
@@ -576,7 +582,7 @@ __global__ void __launch_bounds__(TT, 5) token_logprob_grad_kernel(const GradArg
     };
 
     const int lo = s0 - tid, hi = lo + GU * TT;
-    if (!zero && lo * E - lead - (shift ? E : 0) >= 0 && (hi + (shift ? 1 : 0)) * E - lead <= v) {
+    if (!zero && !far && lo * E - lead - (shift ? E : 0) >= 0 && (hi + (shift ? 1 : 0)) * E - lead <= v) {
         const uint4* from = reinterpret_cast<const uint4*>(p - lead - shift / (int)sizeof(T)) + s0;
         uint4* to = reinterpret_cast<uint4*>(o - lead) + s0;
         uint4 u[GU];
@@ -594,7 +600,7 @@ __global__ void __launch_bounds__(TT, 5) token_logprob_grad_kernel(const GradArg
         for (int i = 0; i < GU; ++i) {
             float x[E];
             unpack(u[i], x, T());
-            gradient(x, s0 + i * TT);
+            gradient(x, s0 + i * TT, false);
             __stcs(to + i * TT, pack(x, T()));
         }
         return;
@@ -607,7 +613,7 @@ __global__ void __launch_bounds__(TT, 5) token_logprob_grad_kernel(const GradArg
             for (int q = 0; q < E; ++q) x[q] = 0.f;
         } else {
             window(p, v, j, shift, x);
-            gradient(x, s);
+            gradient(x, s, far);
         }
         put(o, v, j, x);
     }
@@ -1018,13 +1024,15 @@ __global__ void __launch_bounds__(TT) token_lanes_kernel(const LanesArgs a) {
         const long long t = load_id(a.ids, n, a.wide);
         const float norm = __ldg(a.lse + n), gl = t >= 0 && t < a.v ? __ldg(a.g_logp + n) : 0.f;
         const float gh = a.g_entropy ? __ldg(a.g_entropy + n) : 0.f, h = a.g_entropy ? __ldg(a.entropy + n) : 0.f;
-        const bool zero = norm == NEG_INF || (gl == 0.f && gh == 0.f);
+        const bool zero = norm == NEG_INF || (gl == 0.f && gh == 0.f), far = fabsf(norm) >= FAR_LSE;
         T* g = reinterpret_cast<T*>(a.g) + n * a.g_pitch;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             const int j = lane + i * L;
             if (live && j < a.v) {
-                const float d = fmaf(x[i], a.scale, -norm), pr = ex2(d * LOG2E);
+                float d = fmaf(x[i], a.scale, -norm);
+                if (far && d > 0.f) d = 0.f;
+                const float pr = ex2(d * LOG2E);
                 float r = -a.scale * pr * fmaf(gh, floor_y(d) + h, gl);
                 if (j == t) r += gl * a.scale;
                 g[j] = from_f<T>(zero ? 0.f : r);

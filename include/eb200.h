@@ -121,7 +121,9 @@ typedef enum {
                               * entropy [N] and g_entropy [N] (lse and entropy as the forward kernel left them); output [N, V] in
                               * the logits' type = scalar * (g_logp * ([j = t] - p_j) - g_entropy * p_j * (ln p_j + entropy)), where
                               * g_logp counts as 0 for a padding token.  A row whose g_logp and g_entropy are 0, and a row whose
-                              * lse is -inf, has gradient 0 whatever its logits; K is 0 */
+                              * lse is -inf, has gradient 0 whatever its logits; K is 0.  p_j = exp(x_j - lse) from lse as F32 holds
+                              * it, off by |lse| 2^-24 of itself; where |lse| >= 2^22 (rows of a mask's lowest value) it is at most
+                              * 1, so that the gradient stays finite, and need not sum to 1 */
     EB200_K_DISTILL_TOPK = 12, /* distillation from a teacher's top logits: shape = {N, V, K}, 1 <= K <= 256; inputs logits [N, V]
                               * (F32 / F16 / BF16), the teacher's values [N, K] (F32 / F16 / BF16; logits or log-probabilities) and
                               * their indices [N, K] (I32 / I64).  q = softmax(scalar * values) over the K entries, p = softmax(scalar *

@@ -234,3 +234,33 @@ def test_a_certain_token_has_probability_one(dev, registry, kind, n, v, k):
                                            "f32", 0.9, v + 1, 3)
     assert (loss[one] == 0).all() and (loss2[one] == 0).all() and (loss >= 0).all() and (loss2 >= 0).all(), kerns[0].impl
     assert (grad[one] == 0).all(), kerns[1].impl
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("scale", [1.0, 0.7, 0.45, 0.9])
+@pytest.mark.parametrize("n,v", [(5, 100), (5, 1000), (40, 9001)])
+def test_token_gradient_of_far_rows_stays_finite(dev, registry, kind, scale, n, v):
+    """Rows of nothing but a mask's lowest value, or of huge logits: their lse in 32 bits is coarser than any ln p, but a
+    probability stays within [0, 1], so each gradient within scale * (|g_logp| + |g_entropy| * (1/e + |entropy|))."""
+    rng = np.random.default_rng(v)
+    x = logits(rng, n, v)
+    stored, _ = store(x, kind)
+    stored[0] = {"f32": np.finfo(np.float32).min, "f16": -65504.0, "bf16": 0xFF7F}[kind]
+    stored[1] = stored[0]
+    stored[1, ::2] = 0xFF80 if kind == "bf16" else -np.inf
+    stored[2] = store(np.clip(x[2] * 1e30, -65504, 65504) if kind == "f16" else x[2] * 1e30, kind)[0]
+    stored[3] = store(np.where(x[3] > 0, 3e4, -3e4) if kind == "f16" else np.where(x[3] > 0, 1e38, -1e38), kind)[0]
+    ids = rng.integers(0, v, n)
+    got, _ = run_logprob(dev, registry, stored, ids, 0, kind, scale)
+    gl, gh = rng.standard_normal(n).astype(np.float32), rng.standard_normal(n).astype(np.float32)
+    for entropy in (False, True):
+        ins = [upload(dev, stored, KIND[kind]), upload(dev, ids, D.I32), upload(dev, got["lse"], D.F32), upload(dev, gl, D.F32)]
+        if entropy:
+            ins += [upload(dev, got["entropy"], D.F32), upload(dev, gh, D.F32)]
+        out = upload(dev, store(np.full(n * v, GUARD, np.float32), kind)[0], KIND[kind])
+        kern = registry.compile_ast(dev, D.token_logprob_grad(n, v, entropy, KIND[kind], scale=scale))
+        kern.execute(ins, [out])
+        g = value(out.read_vec(), kind).reshape(n, v)
+        bound = scale * (np.abs(gl) + (np.abs(gh) * (np.exp(-1) + np.abs(got["entropy"])) if entropy else 0)) * (1 + 2 ** -6)
+        assert np.isfinite(g).all(), (kern.impl, np.nonzero(~np.isfinite(g))[0][:4])
+        assert (np.abs(g) <= bound[:, None] + 2 ** -20).all(), (kern.impl, np.abs(g).max(1) / bound)
