@@ -328,11 +328,11 @@ __device__ __forceinline__ Final finish(const Stat& st, float c) {
     f.empty = st.mx == NEG_INF && st.s == 0.f;                  // a NaN makes s NaN
     if (f.empty) { f.s = 1.f; f.ln_s = 0.f; f.mean = 0.f; return f; }
     const float dy = fmaf(st.mx, c, -st.rc), own = ex2(dy), rest = st.s - own;
-    float others = rest / own, mean = LN2 * (fmaf(-dy, rest, st.t - __fmul_rn(own, dy)) / st.s);
+    float others = rest * ex2(-dy), mean = LN2 * (fmaf(-dy, rest, st.t - __fmul_rn(own, dy)) / st.s);
     if (others < 0.f) others = 0.f;                             // NaN stays
     if (mean > 0.f) mean = 0.f;
     f.s = 1.f + others;
-    f.ln_s = log1pf(others);
+    f.ln_s = logf(f.s);                                         // of `others` no digits are left that log1p would keep
     f.mean = mean;
     return f;
 }
@@ -880,7 +880,7 @@ __global__ void __launch_bounds__(RowsShape<MODE>::THREADS, RowsShape<MODE>::CTA
             if (cluster > 1) cluster_wait();
         }
         if (cluster > 1) st = exchange<CT>(st, sh.stat[b], &sh.peers[0], cluster, rank, a.error_flag);
-        Final f;
+        Final f = {};
         if (again<T, ENT>(st.mx, c)) {
             Acc sec(c);
             for (int s = sl.first + tid; s < sl.first + sl.m; s += CT) {
@@ -892,7 +892,7 @@ __global__ void __launch_bounds__(RowsShape<MODE>::THREADS, RowsShape<MODE>::CTA
             Stat st2 = cta_totals<CT>(sec, sh.second);
             if (cluster > 1) st2 = exchange<CT>(st2, sh.second, &sh.peers[1], cluster, rank, a.error_flag);
             f = finish_against(st2, st.mx);
-        } else {
+        } else if (MODE != ROWS_LOGPROB || warp == 0) {             // without alternatives one thread writes
             f = finish(st, c);
         }
 
