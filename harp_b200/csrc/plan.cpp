@@ -292,7 +292,8 @@ static int plan_token(const eb200_kernel_desc* d, int sm_count, Plan* plan) {
         if (role == 0) {
             EB_REQUIRE(is_float(o.dtype) && (!out || o.dtype == t.dtype), EB200_ERR_UNSUPPORTED, "%s: logits are F32, F16 or BF16, the gradient of the same type", what);
             const long long pitch = o.strides[0] == 0 ? V : o.strides[0];
-            EB_REQUIRE(pitch >= V && pitch < (1LL << 32) && (o.strides[1] == 1 || o.strides[1] == 0), EB200_ERR_UNSUPPORTED,
+            const bool unit = o.strides[1] == 1 || (o.strides[1] == 0 && (o.strides[0] == 0 || V == 1));
+            EB_REQUIRE(pitch >= V && pitch < (1LL << 32) && unit && o.strides[2] == 0, EB200_ERR_UNSUPPORTED,
                        "%s operand %d: rows are contiguous and at least %lld elements apart", what, i, V);
             need = N ? (N - 1) * pitch + V : 0;
             (out ? t.g_pitch : t.pitch) = pitch;
@@ -305,6 +306,13 @@ static int plan_token(const eb200_kernel_desc* d, int sm_count, Plan* plan) {
             t.teacher_dtype = o.dtype;
         } else {
             EB_REQUIRE(o.dtype == EB200_F32, EB200_ERR_UNSUPPORTED, "%s operand %d is F32", what, i);
+        }
+        if (role != 0) {
+            // dense: no strides at all, those of the operand's own [N] or [N, K], or K's in the place of shape[2]
+            const long long per = need / std::max(N, 1LL), s0 = o.strides[0], s1 = o.strides[1], s2 = o.strides[2];
+            const bool rows = s0 == per || N <= 1, none = s0 == 0 && s1 == 0 && s2 == 0;
+            EB_REQUIRE(none || (rows && (per > 1 ? s1 + s2 == 1 && (s1 == 0 || s2 == 0) : (s1 == 0 || s1 == 1) && (s2 == 0 || s2 == 1))),
+                       EB200_ERR_UNSUPPORTED, "%s operand %d is dense", what, i);
         }
         EB_REQUIRE(o.numel >= need && o.offset <= o.numel - need, EB200_ERR_BOUNDS, "%s operand %d too small", what, i);
         if (out) {

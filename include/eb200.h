@@ -135,7 +135,8 @@ typedef enum {
                               * Of both classes: the logits, and the gradient as the descriptor's `output`, may have any row pitch
                               * >= V (strides[0]; 0 = V), unit column stride and any offset; `output` describes the gradient where
                               * the kernel writes one (its last output) and output 0 otherwise.  All other operands are dense
-                              * and, except output 0 of a forward kernel and the inputs, start at element 0.  N may be 0.  Results
+                              * (strides all 0, or the dense ones; others are refused) and, except output 0 of a forward kernel
+                              * and the inputs, start at element 0.  N may be 0.  Results
                               * do not depend on what else runs: no atomics on memory, one launch, no scratch */
     EB200_K_ADAM = 8         /* Adam::step (crates/nn/src/optim/adam.rs:104-147): inputs p, g, m, v and a one-element
                               * I32 step counter t; the output receives p; m, v and t are updated IN PLACE (t <- t + 1

@@ -129,3 +129,48 @@ def test_refusals(desc, fields, status):
     with pytest.raises(capi.Eb200Error) as e:
         query(changed(desc, **fields))
     assert e.value.status == status and e.value.message
+
+
+STEP_OVER = D.token_logprob(8, 100, 0, stride=120)
+
+
+@pytest.mark.parametrize("desc,fields", [
+    (LP, {"inputs__1__strides__0": 2}),                            # tokens two elements apart
+    (LP, {"inputs__1__strides__0": -1}),
+    (LP, {"inputs__1__strides__1": 3}),
+    (LP, {"output__strides__0": 2}),
+    (GR, {"inputs__2__strides__0": 7}),
+    (GR, {"inputs__3__strides__0": 4}),
+    (GR, {"inputs__4__strides__0": 2}),
+    (GR, {"inputs__5__strides__0": 2}),
+    (KD, {"inputs__1__strides__0": 8, "inputs__1__strides__1": 1}),       # teacher rows 8 apart, 5 wide
+    (KD, {"inputs__2__strides__0": 1, "inputs__2__strides__1": 8}),       # transposed
+    (KD, {"inputs__1__strides__0": 5}),                            # one entry for the whole row
+    (KD, {"inputs__1__strides__0": 5, "inputs__1__strides__1": 1, "inputs__1__strides__2": 1}),
+    (KD, {"output__strides__0": 3}),
+    (KG, {"inputs__3__strides__0": 2}),
+    (LP, {"inputs__0__strides__1": 0}),                            # one logit for the whole row, rows 100 apart
+    (STEP_OVER, {"inputs__0__strides__1": 0}),
+    (LP, {"inputs__0__strides__2": 1}),
+    (GR, {"output__strides__1": 0}),
+])
+def test_strides_that_would_not_be_followed_are_refused(desc, fields):
+    """Operands that the kernels take as dense, described otherwise."""
+    query(desc)
+    with pytest.raises(capi.Eb200Error) as e:
+        query(changed(desc, **fields))
+    assert e.value.status == capi.ERR_UNSUPPORTED and e.value.message
+
+
+@pytest.mark.parametrize("desc,fields", [
+    (LP, {"inputs__1__strides__0": 1, "output__strides__0": 1}),
+    (LP, {"inputs__0__strides__0": 0, "inputs__0__strides__1": 0}),
+    (KD, {"inputs__1__strides__0": 5, "inputs__1__strides__1": 1, "inputs__2__strides__0": 5, "inputs__2__strides__2": 1}),
+    (D.distill_topk(8, 100, 1), {"inputs__1__strides__0": 1, "inputs__1__strides__1": 1, "inputs__2__strides__0": 1}),
+    (D.distill_topk(1, 100, 5), {"inputs__1__strides__0": 99, "inputs__1__strides__1": 1}),
+    (D.token_logprob(8, 1), {"inputs__0__strides__1": 0}),
+    (GR, {f"inputs__{i}__strides__0": 1 for i in range(1, 6)}),
+    (KG, {"inputs__3__strides__0": 1}),
+])
+def test_dense_operands_may_say_so(desc, fields):
+    query(changed(desc, **fields))
