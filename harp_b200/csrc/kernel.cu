@@ -31,6 +31,8 @@ int find_chain(const KInsn* prog, int n_insns) {
 }
 
 static int dtype_bytes(int dt) { return dt == EB200_BOOL ? 1 : dt == EB200_I64 ? 8 : (dt == EB200_F16 || dt == EB200_BF16) ? 2 : 4; }
+// by division: a descriptor may name any number of elements, and a product of 64 bits would wrap
+static bool holds(size_t bytes, long long numel, int dt) { return numel >= 0 && (size_t)numel <= bytes / dtype_bytes(dt); }
 
 }  // namespace eb200
 
@@ -88,19 +90,17 @@ int eb200_kernel_launch(eb200_kernel* k, eb200_buffer* const* inputs, int n_inpu
     Device* dev = k->dev;
     for (int i = 0; i < n_inputs; ++i) {
         EB_REQUIRE(inputs[i] && inputs[i]->dev == dev, EB200_ERR_INVALID, "input %d is null or lives on another device", i);
-        size_t need = (size_t)plan.in_numel[i] * dtype_bytes(plan.in_dtype[i]);
-        EB_REQUIRE(inputs[i]->bytes >= need, EB200_ERR_BOUNDS, "input %d holds %zu bytes, kernel addresses %zu", i, inputs[i]->bytes, need);
+        EB_REQUIRE(holds(inputs[i]->bytes, plan.in_numel[i], plan.in_dtype[i]), EB200_ERR_BOUNDS, "input %d holds %zu bytes, kernel addresses %lld elements of %d", i,
+                   inputs[i]->bytes, (long long)plan.in_numel[i], dtype_bytes(plan.in_dtype[i]));
     }
     eb200_buffer* ob = outputs[0];
     EB_REQUIRE(ob && ob->dev == dev, EB200_ERR_INVALID, "output is null or lives on another device");
-    {
-        size_t need = (size_t)plan.out_numel * dtype_bytes(plan.out_dtype);
-        EB_REQUIRE(ob->bytes >= need, EB200_ERR_BOUNDS, "output holds %zu bytes, kernel addresses %zu", ob->bytes, need);
-    }
+    EB_REQUIRE(holds(ob->bytes, plan.out_numel, plan.out_dtype), EB200_ERR_BOUNDS, "output holds %zu bytes, kernel addresses %lld elements of %d", ob->bytes,
+               (long long)plan.out_numel, dtype_bytes(plan.out_dtype));
     for (int j = 1; j < n_outputs; ++j) {
         EB_REQUIRE(outputs[j] && outputs[j]->dev == dev, EB200_ERR_INVALID, "output %d is null or lives on another device", j);
-        size_t need = (size_t)plan.more_numel[j - 1] * dtype_bytes(plan.more_dtype[j - 1]);
-        EB_REQUIRE(outputs[j]->bytes >= need, EB200_ERR_BOUNDS, "output %d holds %zu bytes, kernel addresses %zu", j, outputs[j]->bytes, need);
+        EB_REQUIRE(holds(outputs[j]->bytes, plan.more_numel[j - 1], plan.more_dtype[j - 1]), EB200_ERR_BOUNDS,
+                   "output %d holds %zu bytes, kernel addresses %lld elements of %d", j, outputs[j]->bytes, (long long)plan.more_numel[j - 1], dtype_bytes(plan.more_dtype[j - 1]));
     }
     EB_CHECK_CUDA(cudaSetDevice(dev->index));
     // the output may share storage with a clone: give it its own, keeping the

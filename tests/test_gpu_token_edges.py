@@ -264,3 +264,24 @@ def test_token_gradient_of_far_rows_stays_finite(dev, registry, kind, scale, n, 
         bound = scale * (np.abs(gl) + (np.abs(gh) * (np.exp(-1) + np.abs(got["entropy"])) if entropy else 0)) * (1 + 2 ** -6)
         assert np.isfinite(g).all(), (kern.impl, np.nonzero(~np.isfinite(g))[0][:4])
         assert (np.abs(g) <= bound[:, None] + 2 ** -20).all(), (kern.impl, np.abs(g).max(1) / bound)
+
+
+@pytest.mark.parametrize("many", [1 << 61, 1 << 62, (1 << 62) + 5, (1 << 63) - 1])
+def test_more_elements_than_64_bits_of_bytes_are_refused(dev, registry, many):
+    """A descriptor may name more elements than any buffer holds; their bytes wrap around 64 bits."""
+    f = lambda m, t=D.F32: upload(dev, np.zeros(m), t)       # noqa: E731
+    ins, outs = [f(400), f(4, D.I32)], [f(4) for _ in range(3)]
+    small = [f(1), f(1, D.I32)], [f(1) for _ in range(3)]
+    for which in range(3):
+        d = D.token_logprob(4, 100)
+        (d.inputs + [d.output])[which].numel = many
+        kern = registry.compile_ast(dev, d)
+        for i, o in ((ins, outs), small):
+            with pytest.raises(capi.Eb200Error) as e:
+                kern.execute(i, o)
+            assert e.value.status == capi.ERR_BOUNDS, e.value.message
+    d = D.distill_topk(4, 100, 1, grad=True)
+    d.output.numel = many
+    with pytest.raises(capi.Eb200Error) as e:
+        registry.compile_ast(dev, d).execute([f(400), f(4), f(4, D.I32), f(4)], [f(4), f(400)])
+    assert e.value.status == capi.ERR_BOUNDS, e.value.message
