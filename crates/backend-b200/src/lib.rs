@@ -167,10 +167,13 @@ impl Kernel for B200Kernel {
             let buf = buf.as_any().downcast_ref::<B200Buffer>().ok_or_else(|| dyn_err("B200Kernel requires B200Buffer arguments".into()))?;
             ins.push(buf.handle);
         }
-        if outputs.len() != 1 { return Err(dyn_err(format!("kernel writes 1 output, {} given", outputs.len()))); }
-        let out = outputs[0].as_any().downcast_ref::<B200Buffer>().ok_or_else(|| dyn_err("B200Kernel requires B200Buffer arguments".into()))?;
-        let outs = [out.handle];
-        ffi::check(unsafe { ffi::eb200_kernel_launch(self.handle, ins.as_ptr(), ins.len() as i32, outs.as_ptr(), 1) }).map_err(dyn_err)
+        // how many outputs a class writes is the library's check (a token log-probability kernel writes 3 or 5)
+        let mut outs: Vec<*mut ffi::eb200_buffer> = Vec::with_capacity(outputs.len());
+        for out in outputs.iter() {
+            let out = out.as_any().downcast_ref::<B200Buffer>().ok_or_else(|| dyn_err("B200Kernel requires B200Buffer arguments".into()))?;
+            outs.push(out.handle);
+        }
+        ffi::check(unsafe { ffi::eb200_kernel_launch(self.handle, ins.as_ptr(), ins.len() as i32, outs.as_ptr(), outs.len() as i32) }).map_err(dyn_err)
     }
 
     fn execute_with_sizes(&self, inputs: &[&dyn Buffer], outputs: &mut [&mut dyn Buffer], _grid: [usize; 3], _local: [usize; 3]) -> Result<(), DynError> {

@@ -63,3 +63,18 @@ def test_no_device_is_an_error_not_a_fallback():
     st = capi.load().eb200_device_open(0, C.byref(h))
     assert st == capi.ERR_NO_DEVICE
     assert capi.load().eb200_last_error()
+
+
+def test_crate_hands_over_every_buffer_and_names_the_classes_alike():
+    """The Rust binding, read as text (there is no toolchain to compile it): a launch passes as many inputs and outputs as
+    it was given, and the kernel classes have the header's numbers."""
+    crate = os.path.join(ROOT, "crates", "backend-b200", "src")
+    lib = open(os.path.join(crate, "lib.rs")).read()
+    calls = re.findall(r"eb200_kernel_launch\((.*?)\) \}", lib)
+    assert calls and all("ins.len() as i32" in c and "outs.len() as i32" in c for c in calls)
+    assert "outputs.len() != 1" not in lib
+    header = open(os.path.join(ROOT, "include", "eb200.h")).read()
+    ffi = open(os.path.join(crate, "ffi.rs")).read()
+    theirs = {n: int(v) for n, v in re.findall(r"pub const (K_[A-Z0-9_]+): i32 = (\d+);", ffi)}
+    ours = {n: int(v) for n, v in re.findall(r"EB200_(K_[A-Z0-9_]+) = (\d+)", header)}
+    assert theirs == ours and len(ours) == 13
