@@ -1206,7 +1206,8 @@ int launch_lanes_of(Device* dev, const Plan& plan, const LanesArgs& a, size_t sm
     const long long blocks = (a.rows + TT / L - 1) / (TT / L);
     switch (plan.impl) {
         case IMPL_TOKEN_LOGPROB: return launch_rows(dev, token_lanes_kernel<T, L, E, LANES_LOGPROB>, blocks, 1, 0, a);
-        case IMPL_TOKEN_LOGPROB_GRAD: return launch_rows(dev, token_lanes_kernel<T, L, E, LANES_GRAD>, blocks, 1, 0, a);
+        case IMPL_TOKEN_LOGPROB_GRAD:
+            if constexpr (L * E <= 256) return launch_rows(dev, token_lanes_kernel<T, L, E, LANES_GRAD>, blocks, 1, 0, a);
         default: break;
     }
     if (plan.tok.grad) return launch_rows(dev, token_lanes_kernel<T, L, E, LANES_DISTILL_GRAD>, blocks, 1, smem, a);
