@@ -479,7 +479,8 @@ def distill_topk(n: int, v: int, k: int, grad: bool = False, dtype: int = F32, t
     """Distillation from a teacher's `k` top logits per row: KL(softmax(scale * teacher values) || softmax(scale
     * logits) at the teacher's indices).  Inputs: logits [n, v], teacher values [n, k] and indices [n, k] (outside
     [0, v): no entry); output: loss [n].  With `grad` a fourth input, row weights [n], and a second output: the
-    gradient of sum(weights * loss), [n, v] in the logits' type."""
+    gradient of sum(weights * loss), [n, v] in the logits' type.  ``token_logprob`` alternatives at scale 1 can be the
+    teacher's values, whatever `scale` is here (it applies to both sides)."""
     ins = [_rows(n, v, dtype, stride, offset), _dense(n * k, teacher_dtype), _dense(n * k, ids_dtype)] + ([_dense(n)] if grad else [])
     return KernelDesc(K_DISTILL_TOPK, [n, v, k], ins, _rows(n, v, dtype, grad_stride, grad_offset) if grad else _dense(n), None,
                       scalar=scale, flags=FLAG_TOKEN_GRAD if grad else 0)

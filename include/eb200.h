@@ -128,7 +128,9 @@ typedef enum {
                               * (F32 / F16 / BF16), the teacher's values [N, K] (F32 / F16 / BF16; logits or log-probabilities) and
                               * their indices [N, K] (I32 / I64).  q = softmax(scalar * values) over the K entries, p = softmax(scalar *
                               * logits) over all V; output loss [N] F32 = sum_k q_k (ln q_k - ln p[index_k]).  Entries whose
-                              * index is outside [0, V) or whose value is -inf do not take part; a row without entries has loss
+                              * index is outside [0, V) or whose value is -inf do not take part.  The alternatives of
+                              * EB200_K_TOKEN_LOGPROB at scalar 1 serve as values for any scalar here; those of a pass at another
+                              * scalar are scaled already and would be scaled twice.  A row without entries has loss
                               * 0 and gradient 0; an index may occur more than once.  Flags bit 7: loss and gradient in one kernel;
                               * a fourth input, weights [N] F32; outputs loss [N] and the gradient [N, V] (the logits' type) of
                               * sum_n weight_n * loss_n.  A row of weight 0, and a row of -inf logits, has gradient 0.

@@ -285,3 +285,32 @@ def test_more_elements_than_64_bits_of_bytes_are_refused(dev, registry, many):
     with pytest.raises(capi.Eb200Error) as e:
         registry.compile_ast(dev, d).execute([f(400), f(4), f(4, D.I32), f(4)], [f(4), f(400)])
     assert e.value.status == capi.ERR_BOUNDS, e.value.message
+
+
+@pytest.mark.parametrize("temperature", [1.0, 2.0, 0.5])
+@pytest.mark.parametrize("n,v,k", [(9, 700, 12), (37, 5003, 16)])
+def test_alternatives_as_the_teacher_at_a_temperature(dev, registry, temperature, n, v, k):
+    """A teacher's alternatives from a pass at scale 1, distilled at another temperature: the targets are the teacher's
+    logits softened once."""
+    rng = np.random.default_rng(5)
+    teacher, student = logits(rng, n, v), logits(rng, n, v)
+    got, _ = run_logprob(dev, registry, teacher, np.zeros(n, np.int64), k, "f32")
+    scale = 1.0 / temperature
+    w = np.full(n, 1.0 / n, np.float32)
+    loss, loss2, grad, _ = run_distill(dev, registry, student, got["top"], got["top_ids"], w, "f32", "f32", scale)
+    own = np.take_along_axis(teacher, got["top_ids"], 1)
+    want, tol = R.distill(student, own, got["top_ids"], scale, w)
+    # the values come from the kernel: each off by its own tolerance e, which moves ln q by at most 2 scale e, q by that
+    # part of itself, and the loss by sum q |ln q - ln p| of it and the change of ln q itself
+    slack = 2 * scale * R.logprob(teacher, np.zeros(n, np.int64), k)[1]["top"].max()
+    x = student.astype(np.float64) * scale
+    ln_p = np.take_along_axis(x, got["top_ids"], 1) - np.log(np.exp(x).sum(1))[:, None]
+    u = own.astype(np.float64) * scale
+    q = np.exp(u) / np.exp(u).sum(1, keepdims=True)
+    moved = slack * (1 + (q * np.abs(np.log(q) - ln_p)).sum(1))
+    near(loss, want["loss"], tol["loss"] + moved, "loss")
+    near(loss2, want["loss"], tol["loss"] + moved, "loss")
+    near(grad, want["grad"], tol["grad"] + slack * scale * w[:, None], "gradient")
+    if temperature != 1.0:                                  # softening in both passes is another target altogether
+        twice, _ = run_logprob(dev, registry, teacher, np.zeros(n, np.int64), k, "f32", scale)
+        assert np.abs(run_distill(dev, registry, student, twice["top"], twice["top_ids"], w, "f32", "f32", scale)[0] - want["loss"]).min() > moved.max()
