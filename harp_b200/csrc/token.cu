@@ -3,8 +3,9 @@
 //
 // With x = scale * z, m = max x, S = sum exp(x - m):
 //   logp = (x_t - m) - ln S,  lse = m + ln S,  H = ln S - (sum e_j (x_j - m)) / S,  e_j = exp(x_j - m)
-// one pass over the row gives m, S and sum e_j (x_j - m).  All statistics are f32 whatever the logits' type.  What
-// bounds the pass is DRAM: one exponential, and about five other instructions, per logit against 2 or 4 bytes read.
+// one pass over the row gives m, S and sum e_j (x_j - m).  All statistics are f32 whatever the logits' type.  The pass
+// costs one exponential, and about five other instructions, per logit against 2 or 4 bytes read: f32 rows run at the
+// copy rate, 16-bit rows between it and the latencies of a row's end.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -531,7 +532,9 @@ template <class T> __device__ __forceinline__ void put(T* p, int v, int j, const
 // d_j = scale * (g_l ([j = t] - p_j) - g_H p_j (ln p_j + H)), p_j = exp(x_j - lse): a stream of logits in and a
 // stream of gradients out, cut along 16-byte slots of the output so that stores stay whole whatever the pitches.
 // A CTA takes GU * 256 slots of a row; all of them whole is the rule, and then nothing is tested per slot.  DRAM bounds
-// it: 4096 x 131072 bf16 with the entropy's term takes 359 us, 5.98 TB/s (a warp per 128 slots with tests per slot: 513).
+// it: 4096 x 131072 bf16 with the entropy's term takes 344 us back to back, 362 among other work (6.2 and 5.9 TB/s; a warp
+// per 128 slots with tests per slot: 513).  Rows out of step with their output load every slot twice and shift: 1023 x
+// 50021 f16 takes 43 us, 4.7 TB/s.
 constexpr int GU = 4;
 
 // lse in f32 is off by up to a quarter from here on (rows of a mask's lowest value, logits of millions): x_j - lse may then
@@ -694,11 +697,13 @@ __device__ __forceinline__ float distill_loss(const TeacherShared& sh, const Fin
 // ahead into the next row while this one is being finished, so what is in flight depends neither on registers nor on
 // where a row ends; one warp fetches what else a row needs (the token's logit, the teacher's entries), a row ahead;
 // CT threads take the logits.  Few rows: the CTAs of a cluster share one, each a slice of whole slots.
-// The distillation gradient has the row's chunks brought a second time, which L2 serves: the rows in work at a time are
-// a fraction of it (one CTA per SM; with four, the second reading came from DRAM: 4096 x 131072 bf16 took 620 us, this
-// form 465).  The forward pass of 4096 x 131072 bf16 takes 185 to 208 us (5.2 to 5.8 TB/s; reading 1.07 GB at the copy rate
-// would take 166): exponentials keep their unit about 70 % busy, and 4096 rows are 9.2 turns of 444 CTAs.  Two or four
-// CTAs per SM measured 3 % slower than three.
+// The distillation gradient has the row's chunks brought a second time.  L2 serves that while the rows in work (one CTA
+// per SM, 148 rows) and the gradient written meanwhile fit: 1024 x 131072 bf16 reads 275 MB of DRAM, one reading; at 512 KB
+// a row (f32) it reads 926 MB, so most second readings miss.  4096 x 131072: bf16 445 to 477 us (1.3 to 1.4 times its
+// bytes at the copy rate; with four CTAs per SM, whose second reading missed, 620), f32 997 us (1.5 times).
+// The forward pass of 4096 x 131072 takes 330 us in f32 (6.5 TB/s), 184 to 215 in bf16 (reading 1.07 GB at the copy rate
+// would take 166): the exponentials' unit works in 68 % of an SM's active cycles and 57 % of all, the rest is latency at
+// rows' ends and the tenth turn of 4096 rows on 444 CTAs.  Two and four CTAs per SM came within 3 % of three.
 enum { ROWS_LOGPROB, ROWS_TOP, ROWS_DISTILL, ROWS_DISTILL_GRAD };
 
 struct RowsArgs {
@@ -978,7 +983,8 @@ __global__ void __launch_bounds__(RowsShape<MODE>::THREADS, RowsShape<MODE>::CTA
 // ---- short rows ------------------------------------------------------------------------------------
 // A row of at most L * E logits lies in the registers of L lanes (logit j in lane j % L), so its maximum is known
 // before the first exponential and S is 1 + the others' sum: ln S = log1p keeps its digits on confident rows.
-// 65536 rows of 10: L = 4 lanes a row, 64 rows a CTA, 8 us, launch included (a CTA per row: 547).
+// 65536 rows of 10: L = 4 lanes a row, 64 rows a CTA, 8 us, launch included (a CTA per row: 547).  Alternatives take a
+// round of the warp each, over all registers: meant for a few.
 enum { LANES_LOGPROB, LANES_GRAD, LANES_DISTILL, LANES_DISTILL_GRAD };
 
 struct LanesArgs {
