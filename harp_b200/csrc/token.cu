@@ -1281,6 +1281,11 @@ int launch_typed(Device* dev, const Plan& plan, const void* const* in, void* con
 // Short rows in registers: 4 lanes up to 16 logits, 8 up to 64, a warp up to 256 (the gradient) or 1024 (the rest).
 // A distillation's teacher entries lie in shared memory, so many entries per row want more lanes.
 // Few longer rows: the CTAs of a cluster share one, until the GPU is full or a slice has less than two slots per thread.
+// Both sides of each limit, us: 65536 f32 rows of 16 / 17 logits 6.1 / 8.4, of 64 / 65 8.5 / 22.8; 16384 bf16 rows of 256 /
+// 257 8.5 / 16.6 (registers of the wider shape), of 1024 / 1025 23.6 / 103, with 20 alternatives 174 / 244, distillation
+// 31 / 123, with its gradient 39 / 411; token gradient of 256 / 257 8.4 / 29.  The register forms end where a lane's
+// registers do; a CTA per row beyond pays its joins and barriers per row.  222 / 223 bf16 rows of 65536, clusters of two
+// and none: 12.5 / 12.5.
 void token_variant(TokenShape* t, int sm_count) {
     t->cluster = 1;
     t->lanes = 0;
